@@ -4,8 +4,9 @@ dropout, class log-probabilities and their gradient.
 `run` computes a case in plain torch operations, or, where `own` is true, through
 rustwood_b200.tokens. Conventions shared by both: an id or target outside the table or the
 classes is padding (a zero row, no gradient, log-probability 0); a row of margins that are
-all -inf has lse -inf, log-probabilities -inf, entropy 0 and gradient 0; equal margins rank
-by their index, lowest first.
+all -inf has lse and log-probabilities -inf, log_sum, entropy and gradient 0; equal margins
+rank by their index, lowest first. A row's normaliser is kept as its largest margin and the
+logarithm of the sum of exponentials relative to it, lse = scale * row_max + log_sum.
 """
 import math
 
@@ -151,16 +152,16 @@ def _margins(gen, case):
 
 
 def _saved(x, scale):
-    """What the forward call leaves for its gradient: lse and entropy, in 32 bits."""
-    z = x.float() * scale
-    m = z.amax(dim=1, keepdim=True)
+    """What the forward call leaves for its gradient, in 32 bits: row_max, log_sum, entropy."""
+    m = x.float().amax(dim=1, keepdim=True)
     dead = m == -math.inf
-    e = torch.exp(z.sub_(torch.where(dead, 0.0, m)))
+    d = (x.float() - torch.where(dead, 0.0, m)).mul_(scale)
+    e = torch.exp(d)
     s = e.sum(dim=1, keepdim=True)
-    t = torch.where(e > 0, e.mul_(z), 0.0).sum(dim=1, keepdim=True)
-    lse = torch.where(dead, -math.inf, m + torch.log(s))
-    h = torch.where(dead, 0.0, torch.log(s) - t / s)
-    return lse[:, 0].contiguous(), h[:, 0].contiguous()
+    t = torch.where(e > 0, e.mul_(d), 0.0).sum(dim=1, keepdim=True)
+    log_sum = torch.where(dead, 0.0, torch.log(s))
+    h = torch.where(dead, 0.0, log_sum - t / s)
+    return m[:, 0].contiguous(), log_sum[:, 0].contiguous(), h[:, 0].contiguous()
 
 
 def prepare(case, seed):
@@ -179,7 +180,7 @@ def prepare(case, seed):
     else:
         st["x"], st["target"] = _margins(gen, case)
         if case["op"] == "logprobs_grad":
-            st["lse"], st["h"] = _saved(st["x"], case["scale"])
+            st["m"], st["log_sum"], st["h"] = _saved(st["x"], case["scale"])
             n = case["n"]  # a loss summed over the rows, each with its weight
             st["g"] = -(0.5 + torch.rand(n, generator=gen, device="cuda"))
             st["e"] = 0.01 * torch.rand(n, generator=gen, device="cuda") if case["entropy"] else None
@@ -204,9 +205,10 @@ def run(state):
             return tokens.dropout(ctx, x, case["p"], state["seed"], state["sequence"])
         if op == "logprobs":
             r = tokens.logprobs(ctx, x, state["target"], scale=case["scale"], top_k=case["top_k"])
-            return {"lse": r.lse, "logp": r.logp, "entropy": r.entropy, "top_logp": r.top_logp, "top_index": r.top_index}
-        return tokens.logprobs_grad(ctx, x, state["target"], state["lse"], state["h"], state["g"], state["e"],
-                                    scale=case["scale"])
+            return {"row_max": r.row_max, "log_sum": r.log_sum, "lse": r.lse, "logp": r.logp, "entropy": r.entropy,
+                    "top_logp": r.top_logp, "top_index": r.top_index}
+        return tokens.logprobs_grad(ctx, x, state["target"], state["m"], state["log_sum"], state["h"], state["g"],
+                                    state["e"], scale=case["scale"])
     if op == "embed":
         return _plain_embed(x, state["ids"], case["scale"], DTYPES[case["out"]])
     if op == "embed_grad":
@@ -215,7 +217,8 @@ def run(state):
         return _plain_dropout(x, case["p"], state["seed"], state["sequence"])
     if op == "logprobs":
         return _plain_logprobs(x, state["target"], case["scale"], case["top_k"])
-    return _plain_logprobs_grad(x, state["target"], state["lse"], state["h"], state["g"], state["e"], case["scale"])
+    return _plain_logprobs_grad(x, state["target"], state["m"], state["log_sum"], state["h"], state["g"], state["e"],
+                                case["scale"])
 
 
 def _plain_embed(table, ids, scale, dtype):
@@ -268,36 +271,36 @@ def _plain_dropout(x, p, seed, sequence):
 
 def _plain_logprobs(x, target, scale, top_k):
     n, vocab = x.shape
-    z = x.float() * scale
-    m = z.amax(dim=1, keepdim=True)
+    m = x.float().amax(dim=1, keepdim=True)
     dead = m == -math.inf
-    d = z - torch.where(dead, 0.0, m)
+    d = (x.float() - torch.where(dead, 0.0, m)) * scale
     e = torch.exp(d)
     s = e.sum(dim=1, keepdim=True)
     t = torch.where(e > 0, e * d, 0.0).sum(dim=1, keepdim=True)
-    log_s = torch.log(s)
-    lse = torch.where(dead, -math.inf, m + log_s)
-    entropy = torch.where(dead, 0.0, log_s - t / s)
+    log_sum = torch.where(dead, 0.0, torch.log(s))
+    lse = m * scale + log_sum
+    entropy = torch.where(dead, 0.0, log_sum - t / s)
     target = target.long()
     seen = (target >= 0) & (target < vocab)
-    at = torch.gather(z, 1, torch.where(seen, target, 0)[:, None])
-    logp = torch.where(seen[:, None], torch.where(dead, -math.inf, at - lse), 0.0)
+    logp = torch.gather(d, 1, torch.where(seen, target, 0)[:, None]) - log_sum
+    logp = torch.where(seen[:, None], logp, 0.0)
     # whole-number keys that rank by value, then by the lower index
     bits = (x.float() + 0.0).view(torch.int32)
     order = torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits).long() * (1 << 32)
     key = torch.topk(order + (vocab - 1 - torch.arange(vocab, device=x.device)), top_k, dim=1).values
     top_index = vocab - 1 - (key & 0xFFFFFFFF)
-    top_logp = torch.where(dead, -math.inf, torch.gather(z, 1, top_index) - lse)
-    return {"lse": lse[:, 0], "logp": logp[:, 0], "entropy": entropy[:, 0], "top_logp": top_logp, "top_index": top_index}
+    top_logp = torch.gather(d, 1, top_index) - log_sum
+    return {"row_max": m[:, 0], "log_sum": log_sum[:, 0], "lse": lse[:, 0], "logp": logp[:, 0],
+            "entropy": entropy[:, 0], "top_logp": top_logp, "top_index": top_index}
 
 
-def _plain_logprobs_grad(x, target, lse, h, g, e, scale):
+def _plain_logprobs_grad(x, target, row_max, log_sum, h, g, e, scale):
     n, vocab = x.shape
     target = target.long()
     seen = (target >= 0) & (target < vocab)
-    dead = (lse == -math.inf)[:, None]
+    dead = (row_max == -math.inf)[:, None]
     g = torch.where(seen, g, 0.0)[:, None]
-    logp = x.float() * scale - torch.where(dead, 0.0, lse[:, None])
+    logp = (x.float() - torch.where(dead, 0.0, row_max[:, None])) * scale - log_sum[:, None]
     p = torch.where(dead, 0.0, torch.exp(logp))
     grad = -g * p
     if e is not None:
@@ -335,8 +338,8 @@ def work(case):
     e, n, size = case["n"] * case["vocab"], case["n"], SIZES[case["dtype"]]
     ids = n * int(case["ids"][1:]) // 8
     if op == "logprobs":
-        return {"bytes": e * size + ids + n * 12 + n * case["top_k"] * 12, "flops": 6 * e}
-    return {"bytes": 2 * e * size + ids + n * (16 if case["entropy"] else 8), "flops": (7 if case["entropy"] else 4) * e}
+        return {"bytes": e * size + ids + n * 20 + n * case["top_k"] * 12, "flops": 6 * e}
+    return {"bytes": 2 * e * size + ids + n * (20 if case["entropy"] else 12), "flops": (7 if case["entropy"] else 4) * e}
 
 
 # ---- the definitions in 64 bits --------------------------------------------------------
@@ -380,7 +383,9 @@ def exact(case, seed):
         t = st["target"].long()
         logp = torch.where(t < 0, 0.0, lp.gather(1, t.clamp(min=0)[:, None])[:, 0])
         h = torch.special.entr(lp.exp_()).sum(dim=1)
-        return {"lse": lse, "logp": logp, "entropy": h, "top_logp": top, "top_index": None}
+        m = x.double().amax(dim=1)
+        log_sum = torch.where(torch.isinf(m), 0.0, lse - case["scale"] * m)
+        return {"row_max": m, "log_sum": log_sum, "lse": lse, "logp": logp, "entropy": h, "top_logp": top, "top_index": None}
     # the gradient of sum(g logp + e H) as p times the differences from its mean, with the
     # definition's own lse and entropy
     p = lp.exp()
