@@ -280,6 +280,92 @@ int rw_target_transform(rw_ctx* ctx, float* x_rowmajor, uint64_t n, uint32_t nf,
                         const uint32_t* categorical, uint32_t n_cat, const rw_encoders* enc,
                         uint64_t hash_buckets);
 
+/* ---- token operators ------------------------------------------------------------
+ *
+ * The vector-valued, many-class side of what this library does with categorical columns
+ * and margins: an embedding row per category where rw_target_transform looks up one value
+ * per key, its gradient where rw_target_encode sums labels by key, dropout where the
+ * samplers drop rows by a counter hash, and class log-probabilities where the boosting
+ * loop has the logistic link. No counterpart in the reference (its categories and labels
+ * are scalars, its objectives binary).
+ *
+ * Conventions of these calls, where they differ from the rest of the header:
+ *  - Every buffer is device memory of the context's (first) GPU, aligned to its element
+ *    type; the caller owns it. Rows may be strided: ld_* is the distance between rows in
+ *    elements, at least the row's width. Outputs must not overlap inputs unless said.
+ *  - Work goes to `stream` (a cudaStream_t of that GPU; NULL is the device's default
+ *    stream, rw_ctx_stream(ctx) the context's own). The calls neither synchronise nor
+ *    allocate, so they can be captured into a CUDA graph; outputs are valid when the
+ *    stream has run them. The calling thread's current device is left as it was.
+ *  - Scratch is the caller's: `workspace` of at least the bytes that the matching
+ *    rw_*_workspace call gives, 256-byte aligned, with any contents; it must not be used
+ *    by anything else until the stream has run the call. Calls that may run at the same
+ *    time (two streams, two graphs) need a workspace each.
+ *  - Results do not depend on timing: the same inputs give the same bits. */
+
+/* Element types (f32, bf16, f16) and the types of ids, targets and categories. */
+enum { RW_F32 = 0, RW_BF16 = 1, RW_F16 = 2 };
+enum { RW_I32 = 0, RW_I64 = 1 };
+#define RW_MAX_TOP 32 /* the most alternatives rw_logprobs_device reports per row */
+
+/* Embedding lookup: out[i] = scale * table[ids[i]], n rows of d, the product in f32 and
+ * rounded once to out_type. An id outside 0..vocab-1 (padding, an unseen category) gives a
+ * row of zeros. */
+int rw_embed_device(rw_ctx* ctx, const void* d_table, int32_t table_type, uint64_t vocab,
+                    uint64_t ld_table, const void* d_ids, int32_t id_type, uint64_t n, uint64_t d,
+                    float scale, void* d_out, int32_t out_type, uint64_t ld_out, void* stream);
+
+/* Its gradient: dtable[v] = scale * (the sum of grad[i] over i with ids[i] == v), zero for
+ * rows no id names; with accumulate != 0 the sums are added to the rows that ids name and
+ * the other rows are left as they were. Sums are f32 in an order that depends on ids alone,
+ * rounded once to dtable_type. Ids outside 0..vocab-1 have no gradient. n, vocab < 2^31. */
+int rw_embed_grad_workspace(rw_ctx* ctx, uint64_t n, uint64_t d, uint64_t vocab, uint64_t* bytes);
+int rw_embed_grad_device(rw_ctx* ctx, const void* d_grad, int32_t grad_type, uint64_t ld_grad,
+                         const void* d_ids, int32_t id_type, uint64_t n, uint64_t d,
+                         uint64_t vocab, float scale, int32_t accumulate, void* d_dtable,
+                         int32_t dtable_type, uint64_t ld_dtable, void* d_workspace,
+                         uint64_t workspace_bytes, void* stream);
+
+/* Dropout: y = x / (1 - p) where kept, else 0 (whatever x is there), for [rows][cols]
+ * elements; y may be x. p in [0, 1] is rounded to a multiple of 2^-16, and the scale is
+ * that p's. Whether element e = row * cols + col is kept depends on (seed, sequence, e, p)
+ * alone: 16 bits of Philox4x32-10 with key seed and counter (e / 8, sequence) -- half e % 2
+ * (the low one first) of word (e / 2) % 4 -- are compared with p * 2^16. The gradient is
+ * the same call on the gradient; give every use its own sequence (or seed). */
+int rw_dropout_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t rows, uint64_t cols,
+                      uint64_t ld_x, double p, uint64_t seed, uint64_t sequence, void* d_y,
+                      uint64_t ld_y, void* stream);
+
+/* Log-probabilities of classes from margins x [n][classes], one pass over them. With
+ * m = max x of a row and d_j = scale * (x_j - m), scale > 0 (an inverse temperature):
+ *   row_max m, log_sum log(sum_j e^d_j), lse scale * m + log_sum;
+ *   logp     d_t - log_sum of the row's target t; 0 when t is outside 0..classes-1;
+ *   entropy  of the row's distribution, in nats;
+ *   top_index / top_logp [n][top_k]: the top_k <= min(RW_MAX_TOP, classes) largest margins
+ *            in descending order, the lower index first among equal ones, and their logp.
+ * All outputs are f32 (top_index int64) and nullable; d_targets is needed with d_logp only.
+ * A row whose margins are all -inf has row_max, lse, logp and top_logp -inf, log_sum and
+ * entropy 0. A NaN or +inf among the margins makes log_sum, lse, logp, entropy and top_logp
+ * NaN; NaN ranks above +inf. classes < 2^31. */
+int rw_logprobs_workspace(rw_ctx* ctx, uint64_t n, uint64_t classes, int32_t type, uint32_t top_k,
+                          uint64_t* bytes);
+int rw_logprobs_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n, uint64_t classes,
+                       uint64_t ld_x, float scale, const void* d_targets, int32_t target_type,
+                       uint32_t top_k, float* d_row_max, float* d_log_sum, float* d_lse,
+                       float* d_logp, float* d_entropy, float* d_top_logp, int64_t* d_top_index,
+                       void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* The gradient of sum_i (grad_logp[i] * logp[i] + grad_entropy[i] * entropy[i]) with
+ * respect to the margins, from rw_logprobs_device's row_max, log_sum and (with
+ * d_grad_entropy) entropy. d_targets with d_grad_logp, and d_grad_entropy, are each
+ * nullable. A target outside 0..classes-1 contributes nothing; a row whose row_max is -inf
+ * has a gradient of zeros. dx has the margins' type and may be x (with the same stride). */
+int rw_logprobs_grad_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n,
+                            uint64_t classes, uint64_t ld_x, float scale, const void* d_targets,
+                            int32_t target_type, const float* d_row_max, const float* d_log_sum,
+                            const float* d_entropy, const float* d_grad_logp,
+                            const float* d_grad_entropy, void* d_dx, uint64_t ld_dx, void* stream);
+
 /* ---- host helpers kept from the reference host code --------------------------- */
 
 /* compute_boundaries (src/data.rs:86-146): out[nf*(n_bins-1)]. */

@@ -23,6 +23,9 @@ RW_ERR = {
     -6: "RW_ERR_TIMEOUT",
 }
 RW_OBJ_LOGISTIC, RW_OBJ_L2 = 0, 1
+RW_F32, RW_BF16, RW_F16 = 0, 1, 2
+RW_I32, RW_I64 = 0, 1
+RW_MAX_TOP = 32
 CATEGORIES = ["gradients", "zero_hist", "build_hist", "allreduce", "split_gain", "apply_split",
               "update_pred"]
 
@@ -95,6 +98,16 @@ def _load() -> C.CDLL:
         "rw_encoders_free": (None, [vp]),
         "rw_encoders_create": (i32, [u32, vp, vp, vp, vp, f32, vp]),
         "rw_target_transform": (i32, [vp, vp, u64, u32, vp, u32, vp, u64]),
+        "rw_embed_device": (i32, [vp, vp, i32, u64, u64, vp, i32, u64, u64, f32, vp, i32, u64, vp]),
+        "rw_embed_grad_workspace": (i32, [vp, u64, u64, u64, P(u64)]),
+        "rw_embed_grad_device": (i32, [vp, vp, i32, u64, vp, i32, u64, u64, u64, f32, i32, vp, i32,
+                                       u64, vp, u64, vp]),
+        "rw_dropout_device": (i32, [vp, vp, i32, u64, u64, u64, C.c_double, u64, u64, vp, u64, vp]),
+        "rw_logprobs_workspace": (i32, [vp, u64, u64, i32, u32, P(u64)]),
+        "rw_logprobs_device": (i32, [vp, vp, i32, u64, u64, u64, f32, vp, i32, u32, vp, vp, vp, vp,
+                                     vp, vp, vp, vp, u64, vp]),
+        "rw_logprobs_grad_device": (i32, [vp, vp, i32, u64, u64, u64, f32, vp, i32, vp, vp, vp, vp,
+                                          vp, vp, u64, vp]),
         "rw_compute_boundaries": (None, [vp, u64, u32, u32, u64, i32, vp]),
         "rw_base_score": (f32, [vp, u64, i32]),
         "rw_model_thr_bins": (i32, [P(Model), vp, u32, vp]),
@@ -126,6 +139,8 @@ EXPORTED = [
     "rw_target_encode", "rw_target_encode_device", "rw_encoders_table", "rw_encoders_free",
     "rw_encoders_create", "rw_target_transform", "rw_compute_boundaries", "rw_base_score",
     "rw_model_thr_bins", "rw_compute_boundaries_device", "rw_fit_with_boundaries",
+    "rw_embed_device", "rw_embed_grad_workspace", "rw_embed_grad_device", "rw_dropout_device",
+    "rw_logprobs_workspace", "rw_logprobs_device", "rw_logprobs_grad_device",
     "rw_debug_level_hist", "rw_debug_expf", "rw_debug_binary_version", "rw_debug_level_step",
     "rw_debug_peer_wait", "rw_debug_lonely_rank_ctx", "rw_ctx_peer_failed",
 ]

@@ -377,6 +377,82 @@ inline size_t boundary_scratch_words(uint32_t nf, uint64_t m) {
   return 3 * (size_t)nf * m + (size_t)nf * kSortMaxParts * 256;
 }
 
+// ---- token operators (embed_kernels.cu, logprobs_kernels.cu) -----------------------
+// Device pointers throughout; strides (ld_*) in elements. The launches go to the caller's
+// stream and *nl counts them.
+struct EmbedLaunch {
+  const void* table;  // [vocab] rows of d, ld_table apart
+  uint64_t vocab, ld_table;
+  const void* ids;    // [n]
+  uint64_t n, d;
+  float scale;
+  void* out;          // [n] rows of d, ld_out apart
+  uint64_t ld_out;
+  int table_type, id_type, out_type;
+};
+cudaError_t launch_embed(const EmbedLaunch& a, cudaStream_t s, int* nl);
+
+struct EmbedGradLaunch {
+  const void* grad;  // [n] rows of d, ld_grad apart
+  uint64_t ld_grad;
+  const void* ids;   // [n]
+  uint64_t n, d, vocab;
+  float scale;
+  int accumulate;    // add to dtable's rows instead of overwriting all of them
+  void* dtable;      // [vocab] rows of d, ld_dtable apart
+  uint64_t ld_dtable;
+  int grad_type, id_type, dtable_type;
+};
+uint64_t embed_grad_workspace(uint64_t n, uint64_t d, uint64_t vocab);
+cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStream_t s, int* nl);
+
+struct DropoutLaunch {
+  const void* x;  // [rows] rows of cols, ld_x apart
+  uint64_t rows, cols, ld_x;
+  uint32_t limit;  // an element is kept where its 16 random bits are >= limit (0..65536)
+  float scale;     // 65536 / (65536 - limit)
+  uint64_t seed, sequence;
+  void* y;
+  uint64_t ld_y;
+  int type;
+};
+cudaError_t launch_dropout(const DropoutLaunch& a, cudaStream_t s, int* nl);
+
+constexpr uint32_t kMaxTop = 32;
+struct LogprobsLaunch {
+  const void* x;        // [n] rows of classes, ld_x apart
+  uint64_t n, classes, ld_x;
+  float scale;
+  const void* targets;  // [n] or null
+  uint32_t top_k;       // 0..min(kMaxTop, classes)
+  float* row_max;       // [n] or null
+  float* log_sum;       // [n] or null
+  float* lse;           // [n] or null
+  float* logp;          // [n] or null (then targets is null)
+  float* entropy;       // [n] or null
+  float* top_logp;      // [n][top_k] or null
+  int64_t* top_index;   // [n][top_k] or null
+  int type, target_type;
+};
+uint64_t logprobs_workspace(uint64_t n, uint64_t classes, int type, uint32_t top_k);
+cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream_t s, int* nl);
+
+struct LogprobsGradLaunch {
+  const void* x;
+  uint64_t n, classes, ld_x;
+  float scale;
+  const void* targets;  // [n] or null
+  const float* row_max;       // [n]
+  const float* log_sum;       // [n]
+  const float* entropy;       // [n], with grad_entropy
+  const float* grad_logp;     // [n], with targets
+  const float* grad_entropy;  // [n] or null
+  void* dx;             // [n] rows of classes, ld_dx apart; may be x
+  uint64_t ld_dx;
+  int type, target_type;
+};
+cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, int* nl);
+
 // ---- test hooks ------------------------------------------------------------------
 cudaError_t launch_debug_expf(const float* x, uint64_t n, float* out_rw, float* out_cuda,
                               cudaStream_t s);

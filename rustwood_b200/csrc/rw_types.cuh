@@ -1,0 +1,66 @@
+// Element types of the token operators (embedding, dropout, class log-probabilities):
+// loads that widen to f32 and stores that round once to the output's type.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "rw_internal.cuh"
+
+__device__ __forceinline__ float rw_widen(float v) { return v; }
+__device__ __forceinline__ float rw_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float rw_widen(__half v) { return __half2float(v); }
+// one rounding, to nearest even
+template <typename T>
+__device__ __forceinline__ T rw_round(float v);
+template <>
+__device__ __forceinline__ float rw_round<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 rw_round<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half rw_round<__half>(float v) { return __float2half_rn(v); }
+
+inline size_t rw_type_bytes(int type) { return type == RW_F32 ? 4 : 2; }
+
+// Calls f with a value of the element type `type` names.
+template <typename F>
+inline cudaError_t rw_with_type(int type, F f) {
+  switch (type) {
+    case RW_F32: return f(float{});
+    case RW_BF16: return f(__nv_bfloat16{});
+    case RW_F16: return f(__half{});
+  }
+  return cudaErrorInvalidValue;
+}
+// Calls f with a value of the index type `type` names.
+template <typename F>
+inline cudaError_t rw_with_index(int type, F f) {
+  switch (type) {
+    case RW_I32: return f(int32_t{});
+    case RW_I64: return f(int64_t{});
+  }
+  return cudaErrorInvalidValue;
+}
+
+// A launch whose error is its own (an earlier, unrelated error of the thread stays where
+// it is). dependent: the launch may start while its predecessor on the stream runs; the
+// kernel waits for it (griddepcontrol.wait) before it touches global memory.
+template <typename... KArgs, typename... Args>
+inline cudaError_t rw_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                             bool dependent, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k, KArgs(args)...);
+}

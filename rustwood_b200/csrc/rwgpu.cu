@@ -790,6 +790,273 @@ static cudaError_t upload_h2d(rw_ctx* ctx, void* dst, const void* src, size_t by
 }
 
 // =================================================================================
+// token operators (embed_kernels.cu, logprobs_kernels.cu)
+
+static rw_ctx* first_rank(rw_ctx* ctx);
+
+namespace {
+
+// Makes the context's device current for a scope and puts the caller's back.
+struct DeviceScope {
+  int before = -1;
+  cudaError_t enter(int device) {
+    int now = 0;
+    cudaError_t e = cudaGetDevice(&now);
+    if (e != cudaSuccess || now == device) return e;
+    e = cudaSetDevice(device);
+    if (e == cudaSuccess) before = now;
+    return e;
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+constexpr uint64_t kMaxItems = (1ull << 31) - 1;
+
+bool elem_type_ok(int32_t t) { return t == RW_F32 || t == RW_BF16 || t == RW_F16; }
+bool index_type_ok(int32_t t) { return t == RW_I32 || t == RW_I64; }
+uint64_t elem_bytes(int32_t t) { return t == RW_F32 ? 4 : 2; }
+uint64_t index_bytes(int32_t t) { return t == RW_I32 ? 4 : 8; }
+bool aligned(const void* p, uint64_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+// Why a [rows][cols] matrix at p with stride ld cannot be used, or null.
+const char* matrix_fault(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t elem) {
+  if (rows == 0 || cols == 0) return nullptr;
+  if (!p) return "is NULL";
+  if (!aligned(p, elem)) return "is not aligned to its element type";
+  if (ld < cols) return "has a row stride below its width";
+  if (ld > UINT64_MAX / 16 / rows) return "is too large";
+  return nullptr;
+}
+
+// The frame of a token operator's entry point: `why` says what is wrong with the arguments
+// (null: nothing), `go` launches. No exception leaves it.
+template <typename Check, typename Go>
+int token_call(rw_ctx* ctx, const char* what, Check why, Go go) {
+  try {
+    const std::string fault = why();
+    if (!fault.empty()) return fail(ctx, RW_ERR_ARG, std::string(what) + ": " + fault);
+    if (!ctx) return fail(nullptr, RW_ERR_ARG, std::string(what) + ": context is NULL");
+    rw_ctx* c = first_rank(ctx);
+    DeviceScope scope;
+    cudaError_t e = scope.enter(c->device);
+    int nl = 0;
+    if (e == cudaSuccess) e = go(&nl);
+    c->launches += nl;
+    return e == cudaSuccess ? RW_OK : cuda_fail(ctx, e, what);
+  } catch (...) {
+    return RW_ERR_OOM;
+  }
+}
+
+#define RW_MATRIX(p, rows, cols, ld, elem)                                        \
+  do {                                                                            \
+    const char* _f = matrix_fault((p), (rows), (cols), (ld), (elem));             \
+    if (_f) return std::string(#p " ") + _f;                                      \
+  } while (0)
+#define RW_VECTOR(p, n, elem) RW_MATRIX(p, n, (uint64_t)1, (uint64_t)1, elem)
+
+std::string workspace_fault(const void* p, uint64_t have, uint64_t need) {
+  if (need == 0) return "";
+  if (!p) return "d_workspace is NULL";
+  if (!aligned(p, 256)) return "d_workspace is not 256-byte aligned";
+  if (have < need)
+    return "the workspace has " + std::to_string(have) + " bytes, " + std::to_string(need) +
+           " are needed";
+  return "";
+}
+
+}  // namespace
+
+extern "C" int rw_embed_device(rw_ctx* ctx, const void* d_table, int32_t table_type, uint64_t vocab,
+                               uint64_t ld_table, const void* d_ids, int32_t id_type, uint64_t n,
+                               uint64_t d, float scale, void* d_out, int32_t out_type,
+                               uint64_t ld_out, void* stream) {
+  return token_call(
+      ctx, "rw_embed_device",
+      [&]() -> std::string {
+        if (!elem_type_ok(table_type) || !elem_type_ok(out_type)) return "unknown element type";
+        if (!index_type_ok(id_type)) return "unknown id type";
+        RW_MATRIX(d_table, vocab, d, ld_table, elem_bytes(table_type));
+        RW_VECTOR(d_ids, n, index_bytes(id_type));
+        RW_MATRIX(d_out, n, d, ld_out, elem_bytes(out_type));
+        return "";
+      },
+      [&](int* nl) {
+        EmbedLaunch a = {d_table, vocab,  ld_table, d_ids,      n,       d,
+                         scale,   d_out,  ld_out,   table_type, id_type, out_type};
+        return launch_embed(a, (cudaStream_t)stream, nl);
+      });
+}
+
+extern "C" int rw_embed_grad_workspace(rw_ctx* ctx, uint64_t n, uint64_t d, uint64_t vocab,
+                                       uint64_t* bytes) {
+  if (!bytes) return fail(ctx, RW_ERR_ARG, "bytes is NULL");
+  *bytes = 0;
+  if (n > kMaxItems || vocab > kMaxItems)
+    return fail(ctx, RW_ERR_ARG, "rw_embed_grad_workspace: n and vocab must be below 2^31");
+  *bytes = embed_grad_workspace(n, d, vocab);
+  return RW_OK;
+}
+
+extern "C" int rw_embed_grad_device(rw_ctx* ctx, const void* d_grad, int32_t grad_type,
+                                    uint64_t ld_grad, const void* d_ids, int32_t id_type,
+                                    uint64_t n, uint64_t d, uint64_t vocab, float scale,
+                                    int32_t accumulate, void* d_dtable, int32_t dtable_type,
+                                    uint64_t ld_dtable, void* d_workspace, uint64_t workspace_bytes,
+                                    void* stream) {
+  return token_call(
+      ctx, "rw_embed_grad_device",
+      [&]() -> std::string {
+        if (!elem_type_ok(grad_type) || !elem_type_ok(dtable_type)) return "unknown element type";
+        if (!index_type_ok(id_type)) return "unknown id type";
+        if (n > kMaxItems || vocab > kMaxItems) return "n and vocab must be below 2^31";
+        RW_MATRIX(d_grad, n, d, ld_grad, elem_bytes(grad_type));
+        RW_VECTOR(d_ids, n, index_bytes(id_type));
+        RW_MATRIX(d_dtable, vocab, d, ld_dtable, elem_bytes(dtable_type));
+        return workspace_fault(d_workspace, workspace_bytes, embed_grad_workspace(n, d, vocab));
+      },
+      [&](int* nl) {
+        EmbedGradLaunch a = {d_grad,     ld_grad,  d_ids,      n,         d,       vocab,      scale,
+                             accumulate, d_dtable, ld_dtable, grad_type, id_type, dtable_type};
+        return launch_embed_grad(a, d_workspace, (cudaStream_t)stream, nl);
+      });
+}
+
+extern "C" int rw_dropout_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t rows,
+                                 uint64_t cols, uint64_t ld_x, double p, uint64_t seed,
+                                 uint64_t sequence, void* d_y, uint64_t ld_y, void* stream) {
+  return token_call(
+      ctx, "rw_dropout_device",
+      [&]() -> std::string {
+        if (!elem_type_ok(type)) return "unknown element type";
+        if (!(p >= 0.0 && p <= 1.0)) return "p is not in [0, 1]";
+        RW_MATRIX(d_x, rows, cols, ld_x, elem_bytes(type));
+        RW_MATRIX(d_y, rows, cols, ld_y, elem_bytes(type));
+        if (d_x == d_y && rows > 1 && cols > 0 && ld_x != ld_y)
+          return "in place needs one stride";
+        return "";
+      },
+      [&](int* nl) {
+        DropoutLaunch a = {};
+        a.x = d_x;
+        a.rows = rows;
+        a.cols = cols;
+        a.ld_x = ld_x;
+        a.limit = (uint32_t)std::nearbyint(p * 65536.0);
+        a.scale = a.limit >= 65536 ? 0.0f : (float)(65536.0 / (65536.0 - a.limit));
+        a.seed = seed;
+        a.sequence = sequence;
+        a.y = d_y;
+        a.ld_y = ld_y;
+        a.type = type;
+        return launch_dropout(a, (cudaStream_t)stream, nl);
+      });
+}
+
+extern "C" int rw_logprobs_workspace(rw_ctx* ctx, uint64_t n, uint64_t classes, int32_t type,
+                                     uint32_t top_k, uint64_t* bytes) {
+  if (!bytes) return fail(ctx, RW_ERR_ARG, "bytes is NULL");
+  *bytes = 0;
+  if (!elem_type_ok(type) || top_k > RW_MAX_TOP || classes > kMaxItems)
+    return fail(ctx, RW_ERR_ARG, "rw_logprobs_workspace: bad type, top_k or classes");
+  *bytes = logprobs_workspace(n, classes, type, top_k);
+  return RW_OK;
+}
+
+extern "C" int rw_logprobs_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n,
+                                  uint64_t classes, uint64_t ld_x, float scale,
+                                  const void* d_targets, int32_t target_type, uint32_t top_k,
+                                  float* d_row_max, float* d_log_sum, float* d_lse, float* d_logp,
+                                  float* d_entropy, float* d_top_logp, int64_t* d_top_index,
+                                  void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  return token_call(
+      ctx, "rw_logprobs_device",
+      [&]() -> std::string {
+        if (!elem_type_ok(type)) return "unknown element type";
+        if (!index_type_ok(target_type)) return "unknown target type";
+        if (!(scale > 0.0f && scale <= 3.0e38f)) return "scale is not positive and finite";
+        if (classes > kMaxItems) return "classes must be below 2^31";
+        if (top_k > RW_MAX_TOP || top_k > classes) return "top_k is above RW_MAX_TOP or classes";
+        RW_MATRIX(d_x, n, classes, ld_x, elem_bytes(type));
+        if (d_logp) RW_VECTOR(d_targets, n, index_bytes(target_type));
+        for (const float* o : {d_row_max, d_log_sum, d_lse, d_logp, d_entropy, d_top_logp})
+          if (!aligned(o, 4)) return "an output is not aligned to its element type";
+        if (!aligned(d_top_index, 8)) return "d_top_index is not aligned to its element type";
+        return workspace_fault(d_workspace, workspace_bytes,
+                               logprobs_workspace(n, classes, type, top_k));
+      },
+      [&](int* nl) {
+        LogprobsLaunch a = {};
+        a.x = d_x;
+        a.n = n;
+        a.classes = classes;
+        a.ld_x = ld_x;
+        a.scale = scale;
+        a.targets = d_targets;
+        a.top_k = top_k;
+        a.row_max = d_row_max;
+        a.log_sum = d_log_sum;
+        a.lse = d_lse;
+        a.logp = d_logp;
+        a.entropy = d_entropy;
+        a.top_logp = d_top_logp;
+        a.top_index = d_top_index;
+        a.type = type;
+        a.target_type = target_type;
+        return launch_logprobs(a, d_workspace, (cudaStream_t)stream, nl);
+      });
+}
+
+extern "C" int rw_logprobs_grad_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n,
+                                       uint64_t classes, uint64_t ld_x, float scale,
+                                       const void* d_targets, int32_t target_type,
+                                       const float* d_row_max, const float* d_log_sum,
+                                       const float* d_entropy, const float* d_grad_logp,
+                                       const float* d_grad_entropy, void* d_dx, uint64_t ld_dx,
+                                       void* stream) {
+  return token_call(
+      ctx, "rw_logprobs_grad_device",
+      [&]() -> std::string {
+        if (!elem_type_ok(type)) return "unknown element type";
+        if (!index_type_ok(target_type)) return "unknown target type";
+        if (!(scale > 0.0f && scale <= 3.0e38f)) return "scale is not positive and finite";
+        if (classes > kMaxItems) return "classes must be below 2^31";
+        if (n == 0 || classes == 0) return "";
+        RW_MATRIX(d_x, n, classes, ld_x, elem_bytes(type));
+        RW_MATRIX(d_dx, n, classes, ld_dx, elem_bytes(type));
+        if (d_x == d_dx && n > 1 && ld_x != ld_dx) return "in place needs one stride";
+        RW_VECTOR(d_row_max, n, 4);
+        RW_VECTOR(d_log_sum, n, 4);
+        if (d_grad_logp) RW_VECTOR(d_targets, n, index_bytes(target_type));
+        if (d_grad_entropy) RW_VECTOR(d_entropy, n, 4);
+        for (const float* v : {d_grad_logp, d_grad_entropy})
+          if (!aligned(v, 4)) return "a gradient is not aligned to its element type";
+        return "";
+      },
+      [&](int* nl) {
+        LogprobsGradLaunch a = {};
+        a.x = d_x;
+        a.n = n;
+        a.classes = classes;
+        a.ld_x = ld_x;
+        a.scale = scale;
+        a.targets = d_grad_logp ? d_targets : nullptr;
+        a.row_max = d_row_max;
+        a.log_sum = d_log_sum;
+        a.entropy = d_entropy;
+        a.grad_logp = d_grad_logp;
+        a.grad_entropy = d_grad_entropy;
+        a.dx = d_dx;
+        a.ld_dx = ld_dx;
+        a.type = type;
+        a.target_type = target_type;
+        return launch_logprobs_grad(a, (cudaStream_t)stream, nl);
+      });
+}
+
+// =================================================================================
 // categorical target encoding (encode.cu)
 
 static rw_ctx* first_rank(rw_ctx* ctx);

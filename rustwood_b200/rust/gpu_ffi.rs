@@ -151,6 +151,35 @@ extern "C" {
     pub fn rw_target_transform(ctx: *mut rw_ctx, x_rowmajor: *mut f32, n: u64, nf: u32,
                                categorical: *const u32, n_cat: u32, enc: *const rw_encoders,
                                hash_buckets: u64) -> c_int;
+    pub fn rw_embed_device(ctx: *mut rw_ctx, d_table: *const c_void, table_type: i32, vocab: u64,
+                           ld_table: u64, d_ids: *const c_void, id_type: i32, n: u64, d: u64,
+                           scale: f32, d_out: *mut c_void, out_type: i32, ld_out: u64,
+                           stream: *mut c_void) -> c_int;
+    pub fn rw_embed_grad_workspace(ctx: *mut rw_ctx, n: u64, d: u64, vocab: u64,
+                                   bytes: *mut u64) -> c_int;
+    pub fn rw_embed_grad_device(ctx: *mut rw_ctx, d_grad: *const c_void, grad_type: i32,
+                                ld_grad: u64, d_ids: *const c_void, id_type: i32, n: u64, d: u64,
+                                vocab: u64, scale: f32, accumulate: i32, d_dtable: *mut c_void,
+                                dtable_type: i32, ld_dtable: u64, d_workspace: *mut c_void,
+                                workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn rw_dropout_device(ctx: *mut rw_ctx, d_x: *const c_void, dtype: i32, rows: u64, cols: u64,
+                             ld_x: u64, p: f64, seed: u64, sequence: u64, d_y: *mut c_void,
+                             ld_y: u64, stream: *mut c_void) -> c_int;
+    pub fn rw_logprobs_workspace(ctx: *mut rw_ctx, n: u64, classes: u64, dtype: i32, top_k: u32,
+                                 bytes: *mut u64) -> c_int;
+    pub fn rw_logprobs_device(ctx: *mut rw_ctx, d_x: *const c_void, dtype: i32, n: u64,
+                              classes: u64, ld_x: u64, scale: f32, d_targets: *const c_void,
+                              target_type: i32, top_k: u32, d_row_max: *mut f32,
+                              d_log_sum: *mut f32, d_lse: *mut f32, d_logp: *mut f32,
+                              d_entropy: *mut f32, d_top_logp: *mut f32, d_top_index: *mut i64,
+                              d_workspace: *mut c_void, workspace_bytes: u64,
+                              stream: *mut c_void) -> c_int;
+    pub fn rw_logprobs_grad_device(ctx: *mut rw_ctx, d_x: *const c_void, dtype: i32, n: u64,
+                                   classes: u64, ld_x: u64, scale: f32, d_targets: *const c_void,
+                                   target_type: i32, d_row_max: *const f32, d_log_sum: *const f32,
+                                   d_entropy: *const f32, d_grad_logp: *const f32,
+                                   d_grad_entropy: *const f32, d_dx: *mut c_void, ld_dx: u64,
+                                   stream: *mut c_void) -> c_int;
     pub fn rw_model_thr_bins(m: *const rw_model, cuts: *const f32, n_bins: u32,
                              thr_bin: *mut u16) -> c_int;
     pub fn rw_compute_boundaries_device(ctx: *mut rw_ctx, d_x: *const f32, n: u64, nf: u32,
