@@ -152,20 +152,215 @@ __global__ void __launch_bounds__(kSortThreads) k_token_scatter(SortPass p) {
   }
 }
 
-// One CTA per sorted position; the CTA at the start of a run of equal ids sums the run.
-template <typename TG, typename TD>
-__global__ void __launch_bounds__(256) k_embed_sum(EmbedGradLaunch a, const unsigned long long* pairs) {
-  for (uint64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-    const uint32_t id = (uint32_t)(pairs[i] >> 32);
-    if (id >= a.vocab || (i > 0 && (uint32_t)(pairs[i - 1] >> 32) == id)) continue;
-    TD* row = (TD*)a.dtable + (uint64_t)id * a.ld_dtable;
-    for (uint64_t c = threadIdx.x; c < a.d; c += blockDim.x) {
-      float acc = 0.0f;
-      for (uint64_t j = i; j < a.n && (uint32_t)(pairs[j] >> 32) == id; j++)
-        acc += rw_widen(((const TG*)a.grad)[(uint64_t)(uint32_t)pairs[j] * a.ld_grad + c]);
-      acc *= a.scale;
-      if (a.accumulate) acc += rw_widen(row[c]);
-      row[c] = rw_round<TD>(acc);
+// The sums. The sorted positions are cut into chunks of equal length; a slot of `tx`
+// threads (V columns each) walks one chunk in order with its running sum in registers.
+// A run of equal ids inside one chunk is finished there; a run that crosses chunks leaves
+// an f32 partial sum in each of them, and k_embed_join adds those in the chunks' order. So
+// a frequent id is summed by many slots, and the order of every addition is fixed by the
+// ids and the sizes.
+
+constexpr int kSumThreads = 256;
+constexpr int kSumDepth = 4;    // rows in flight per thread
+constexpr int kZeroRows = 64;   // table rows a zeroing CTA covers
+constexpr int kJoinThreads = 512;
+constexpr int kJoinCols = 128;  // columns of one join (a float4 a lane)
+constexpr uint32_t kNone = 0xffffffffu;
+
+struct ChunkPlan {
+  uint32_t chunk;       // positions a chunk
+  uint32_t chunks;
+  uint32_t tx, slots;   // threads a slot, slots a CTA
+  uint32_t col_blocks;  // CTAs that share a chunk group's columns
+  uint32_t sum_ctas;    // CTAs that sum; the rest zero rows that no id names
+  uint64_t dv;          // vectors a row
+  uint64_t pitch;       // floats of one partial row (a multiple of 4)
+};
+
+__device__ __forceinline__ uint32_t key_of(unsigned long long pair) { return (uint32_t)(pair >> 32); }
+
+// The first of n sorted pairs whose id is at least key.
+__device__ __forceinline__ uint64_t lower_bound(const unsigned long long* pairs, uint64_t n, uint32_t key) {
+  uint64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const uint64_t mid = (lo + hi) / 2;
+    if (key_of(pairs[mid]) < key) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <typename TG, typename TD, int V>
+__global__ void __launch_bounds__(kSumThreads)
+    k_embed_chunks(EmbedGradLaunch a, ChunkPlan cp, const unsigned long long* __restrict__ pairs,
+                   float* __restrict__ partial) {
+  const uint32_t slot = threadIdx.x / cp.tx, lane = threadIdx.x % cp.tx;
+  TD* dtable = (TD*)a.dtable;
+  if (blockIdx.x >= cp.sum_ctas) {  // zero the rows of this block that no id names
+    __shared__ bool s_absent[kZeroRows];
+    const uint64_t first = (uint64_t)(blockIdx.x - cp.sum_ctas) * kZeroRows;
+    if (threadIdx.x < kZeroRows && first + threadIdx.x < a.vocab) {
+      const uint32_t key = (uint32_t)(first + threadIdx.x);
+      const uint64_t at = lower_bound(pairs, a.n, key);
+      s_absent[threadIdx.x] = at == a.n || key_of(pairs[at]) != key;
+    }
+    __syncthreads();
+    if (slot >= cp.slots) return;
+    Pack<TD, V> zero;
+#pragma unroll
+    for (int k = 0; k < V; k++) zero.set(k, 0.0f);
+    for (uint64_t r = slot; r < kZeroRows && first + r < a.vocab; r += cp.slots) {
+      if (!s_absent[r]) continue;
+      TD* row = dtable + (first + r) * a.ld_dtable;
+      for (uint64_t c = lane; c < cp.dv; c += cp.tx) zero.store(row + c * V);
+    }
+    return;
+  }
+  const uint64_t chunk = (uint64_t)(blockIdx.x / cp.col_blocks) * cp.slots + slot;
+  const uint64_t col = (uint64_t)(blockIdx.x % cp.col_blocks) * cp.tx + lane;
+  if (slot >= cp.slots || chunk >= cp.chunks || col >= cp.dv) return;
+  const uint64_t lo = chunk * cp.chunk, hi = min(lo + cp.chunk, a.n);
+  const TG* grad = (const TG*)a.grad + col * V;
+  float acc[V];
+#pragma unroll
+  for (int k = 0; k < V; k++) acc[k] = 0.0f;
+  uint32_t run = key_of(pairs[lo]);
+  bool before = lo > 0 && key_of(pairs[lo - 1]) == run;
+
+  auto flush = [&](bool after) {
+    if (run >= a.vocab) return;
+    if (before || after) {
+      float* p = partial + (chunk * 2 + (before ? 0 : 1)) * cp.pitch + col * V;
+      Pack<float, V> out;
+#pragma unroll
+      for (int k = 0; k < V; k++) out.v[k] = acc[k];
+      out.store(p);
+    } else {
+      TD* p = dtable + run * a.ld_dtable + col * V;
+      Pack<TD, V> out;
+      if (a.accumulate) out.load(p);
+#pragma unroll
+      for (int k = 0; k < V; k++)
+        out.set(k, a.accumulate ? out.get(k) + acc[k] * a.scale : acc[k] * a.scale);
+      out.store(p);
+    }
+  };
+
+  for (uint64_t j = lo; j < hi; j += kSumDepth) {
+    unsigned long long pair[kSumDepth];
+    Pack<TG, V> row[kSumDepth];
+#pragma unroll
+    for (int u = 0; u < kSumDepth; u++) pair[u] = j + u < hi ? pairs[j + u] : ~0ull;
+#pragma unroll
+    for (int u = 0; u < kSumDepth; u++)
+      if (key_of(pair[u]) < a.vocab) row[u].load(grad + (uint64_t)(uint32_t)pair[u] * a.ld_grad);
+#pragma unroll
+    for (int u = 0; u < kSumDepth; u++) {
+      if (j + u >= hi) break;
+      const uint32_t key = key_of(pair[u]);
+      if (key != run) {
+        flush(false);
+        run = key;
+        before = false;
+#pragma unroll
+        for (int k = 0; k < V; k++) acc[k] = 0.0f;
+      }
+      if (key < a.vocab) {
+#pragma unroll
+        for (int k = 0; k < V; k++) acc[k] += row[u].get(k);
+      }
+    }
+  }
+  flush(hi < a.n && key_of(pairs[hi]) == run);
+}
+
+// Adds the partial sums of the runs that cross chunks: CTA (x, y) takes the runs that start
+// in chunks x, x + gridDim.x, .. and the columns of block y. A run of a few chunks is one
+// warp's, a longer one is shared by all warps and their sums are added in order.
+template <typename TD>
+__global__ void __launch_bounds__(kJoinThreads)
+    k_embed_join(EmbedGradLaunch a, ChunkPlan cp, const unsigned long long* __restrict__ pairs,
+                 const float* __restrict__ partial) {
+  constexpr int kWarps = kJoinThreads / 32;
+  constexpr uint32_t kLong = 24;  // chunks from which on a run is shared by the warps
+  __shared__ uint32_t s_first[kJoinThreads], s_last[kJoinThreads];
+  __shared__ uint32_t s_count;
+  __shared__ float4 s_part[kWarps][32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t col = (uint64_t)blockIdx.y * kJoinCols + lane * 4;
+  TD* dtable = (TD*)a.dtable;
+
+  auto row_sum = [&](uint32_t first, uint32_t lo, uint32_t hi) {
+    // partials lo..hi-1 of the run that starts in chunk `first`, in order
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col < cp.pitch) {
+#pragma unroll 8
+      for (uint32_t q = lo; q < hi; q++) {
+        const float4 v = *(const float4*)(partial + ((uint64_t)q * 2 + (q == first ? 1 : 0)) * cp.pitch + col);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+    }
+    return s;
+  };
+  auto finish = [&](uint32_t first, float4 s) {
+    const uint64_t end = min((uint64_t)(first + 1) * cp.chunk, a.n);
+    TD* p = dtable + (uint64_t)key_of(pairs[end - 1]) * a.ld_dtable + col;
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (col + k >= a.d) break;
+      p[k] = rw_round<TD>(a.accumulate ? rw_widen(p[k]) + v[k] * a.scale : v[k] * a.scale);
+    }
+  };
+
+  for (uint64_t base = 0; base < cp.chunks; base += (uint64_t)gridDim.x * kJoinThreads) {
+    __syncthreads();
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    const uint64_t c = base + blockIdx.x + (uint64_t)threadIdx.x * gridDim.x;
+    if (c + 1 < cp.chunks) {
+      const uint64_t lo = c * cp.chunk, hi = lo + cp.chunk;
+      const uint32_t key = key_of(pairs[hi - 1]);
+      if (key < a.vocab && key_of(pairs[hi]) == key && (lo == 0 || key_of(pairs[lo - 1]) != key)) {
+        // the last chunk that begins with this id
+        uint64_t in = c + 1, out = cp.chunks;
+        while (out - in > 1) {
+          const uint64_t mid = (in + out) / 2;
+          if (key_of(pairs[mid * cp.chunk]) == key) in = mid;
+          else out = mid;
+        }
+        const uint32_t at = atomicAdd(&s_count, 1u);  // the list's order does not matter
+        s_first[at] = (uint32_t)c;
+        s_last[at] = (uint32_t)in;
+      }
+    }
+    __syncthreads();
+    const uint32_t count = s_count;
+    for (uint32_t k = warp; k < count; k += kWarps) {
+      const uint32_t first = s_first[k], last = s_last[k];
+      if (last - first < kLong) finish(first, row_sum(first, first, last + 1));
+    }
+    for (uint32_t k = 0; k < count; k++) {
+      const uint32_t first = s_first[k], last = s_last[k];
+      if (last - first < kLong) continue;
+      const uint32_t m = last + 1 - first, per = (m + kWarps - 1) / kWarps;
+      const uint32_t lo = min(m, warp * per), hi = min(m, lo + per);
+      s_part[warp][lane] = row_sum(first, first + lo, first + hi);
+      __syncthreads();
+      if (warp == 0) {
+        float4 s = s_part[0][lane];
+        for (int w = 1; w < kWarps; w++) {
+          const float4 v = s_part[w][lane];
+          s.x += v.x;
+          s.y += v.y;
+          s.z += v.z;
+          s.w += v.w;
+        }
+        finish(first, s);
+      }
+      __syncthreads();
     }
   }
 }
@@ -248,14 +443,33 @@ cudaError_t launch_embed(const EmbedLaunch& a, cudaStream_t s, int* nl) {
 
 namespace {
 
-// Sizes and workspace offsets of one gradient call.
+// Sizes and workspace offsets of one gradient call. The workspace covers either vector
+// width: it depends on n, d and vocab alone.
 struct GradPlan {
   uint64_t part;
   uint32_t parts, passes;
-  uint64_t pairs0, pairs1, counts, bytes;  // offsets
+  uint64_t pairs0, pairs1, counts, partial, bytes;  // offsets
 };
 
-GradPlan grad_plan(uint64_t n, uint64_t vocab) {
+// Chunks: enough for about 16 CTAs an SM, so that the longest one does not decide the
+// time, but no shorter than 8 positions (the partial sums would be more than a quarter of
+// the traffic) and no more than 32768 (k_embed_join looks at each).
+ChunkPlan chunk_plan(uint64_t n, uint64_t d, int V) {
+  ChunkPlan c = {};
+  c.dv = (d + V - 1) / V;
+  c.tx = (uint32_t)std::min<uint64_t>(c.dv, kSumThreads);
+  c.slots = kSumThreads / c.tx;
+  c.col_blocks = (uint32_t)((c.dv + c.tx - 1) / c.tx);
+  c.pitch = (d + 3) / 4 * 4;
+  const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * 16 * c.slots / c.col_blocks);
+  const uint64_t most = std::min<uint64_t>(want, 32768);
+  c.chunk = (uint32_t)std::max<uint64_t>(8, (n + most - 1) / most);
+  c.chunks = (uint32_t)((n + c.chunk - 1) / c.chunk);
+  c.sum_ctas = (c.chunks + c.slots - 1) / c.slots * c.col_blocks;
+  return c;
+}
+
+GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
   GradPlan g;
   const uint64_t tiles = (n + kSortTile - 1) / kSortTile;
   const uint64_t per = std::max<uint64_t>(1, (tiles + kSms - 1) / kSms);
@@ -273,6 +487,9 @@ GradPlan grad_plan(uint64_t n, uint64_t vocab) {
   g.pairs0 = take(n * 8);
   g.pairs1 = take(n * 8);
   g.counts = take((uint64_t)g.parts * kRadix * 4);
+  const uint64_t chunks =
+      std::max({chunk_plan(n, d, 1).chunks, chunk_plan(n, d, 4).chunks, chunk_plan(n, d, 8).chunks});
+  g.partial = take(chunks * 2 * ((d + 3) / 4 * 4) * 4);
   g.bytes = at;
   return g;
 }
@@ -280,22 +497,22 @@ GradPlan grad_plan(uint64_t n, uint64_t vocab) {
 }  // namespace
 
 uint64_t embed_grad_workspace(uint64_t n, uint64_t d, uint64_t vocab) {
-  return n == 0 || d == 0 || vocab == 0 ? 0 : grad_plan(n, vocab).bytes;
+  return n == 0 || d == 0 || vocab == 0 ? 0 : grad_plan(n, d, vocab).bytes;
 }
 
 cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStream_t s, int* nl) {
   if (a.d == 0 || a.vocab == 0) return cudaSuccess;
   cudaError_t e = cudaSuccess;
-  if (!a.accumulate) {
+  if (a.n == 0) {
+    if (a.accumulate) return cudaSuccess;
     *nl += 1;
-    e = rw_with_type(a.dtable_type, [&](auto td) {
+    return rw_with_type(a.dtable_type, [&](auto td) {
       using TD = decltype(td);
       return rw_launch(k_zero_rows<TD>, dim3(grid_of(a.vocab, 8)), dim3(256), 0, s, false,
                        (TD*)a.dtable, a.vocab, a.d, a.ld_dtable);
     });
   }
-  if (a.n == 0 || e != cudaSuccess) return e;
-  const GradPlan g = grad_plan(a.n, a.vocab);
+  const GradPlan g = grad_plan(a.n, a.d, a.vocab);
   char* ws = (char*)workspace;
   unsigned long long* buf[2] = {(unsigned long long*)(ws + g.pairs0),
                                 (unsigned long long*)(ws + g.pairs1)};
@@ -322,12 +539,32 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
     });
   }
   if (e != cudaSuccess) return e;
-  *nl += 1;
-  return rw_with_type(a.grad_type, [&](auto tg) {
+  const unsigned long long* pairs = buf[(g.passes + 1) & 1];
+  float* partial = (float*)(ws + g.partial);
+  *nl += 2;
+  ChunkPlan cp = {};
+  e = rw_with_type(a.grad_type, [&](auto tg) {
     return rw_with_type(a.dtable_type, [&](auto td) {
-      return rw_launch(k_embed_sum<decltype(tg), decltype(td)>, dim3(grid_of(a.n, 8)), dim3(256), 0,
-                       s, false, a, (const unsigned long long*)buf[(g.passes + 1) & 1]);
+      using TG = decltype(tg);
+      using TD = decltype(td);
+      constexpr int kV = 16 / sizeof(TG);
+      const bool wide = rw_packs(a.grad, a.n, a.d, a.ld_grad, sizeof(TG), kV) &&
+                        rw_packs(a.dtable, a.vocab, a.d, a.ld_dtable, sizeof(TD), kV);
+      cp = chunk_plan(a.n, a.d, wide ? kV : 1);
+      const uint64_t zero = a.accumulate ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
+      const dim3 grid((uint32_t)(cp.sum_ctas + zero));
+      return wide ? rw_launch(k_embed_chunks<TG, TD, kV>, grid, dim3(kSumThreads), 0, s, false, a, cp,
+                              pairs, partial)
+                  : rw_launch(k_embed_chunks<TG, TD, 1>, grid, dim3(kSumThreads), 0, s, false, a, cp,
+                              pairs, partial);
     });
+  });
+  if (e != cudaSuccess) return e;
+  const uint32_t cols = (uint32_t)((a.d + kJoinCols - 1) / kJoinCols);
+  const uint32_t gx = std::max(1u, std::min(cp.chunks, (uint32_t)kSms * 4 / cols));
+  return rw_with_type(a.dtable_type, [&](auto td) {
+    return rw_launch(k_embed_join<decltype(td)>, dim3(gx, cols), dim3(kJoinThreads), 0, s, false, a,
+                     cp, pairs, (const float*)partial);
   });
 }
 

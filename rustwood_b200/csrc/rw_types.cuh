@@ -24,6 +24,55 @@ __device__ __forceinline__ __nv_bfloat16 rw_round<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half rw_round<__half>(float v) { return __float2half_rn(v); }
 
+// V consecutive elements as they lie in memory, moved in pieces of at most 16 bytes; the
+// address is a multiple of a piece.
+template <typename T, int V>
+struct Pack {
+  static constexpr int kBytes = (int)sizeof(T) * V;
+  static constexpr int kPiece = kBytes < 16 ? kBytes : 16;
+  static constexpr int kPieces = kBytes / kPiece;
+  union alignas(kPiece) {
+    T v[V];
+    uint4 q[kBytes >= 16 ? kPieces : 1];
+    uint2 d;
+    uint32_t w;
+    uint16_t h;
+  };
+  __device__ __forceinline__ Pack() {}
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int i = 0; i < kPieces; i++) q[i] = ((const uint4*)p)[i];
+    } else if constexpr (kBytes == 8) {
+      d = *(const uint2*)p;
+    } else if constexpr (kBytes == 4) {
+      w = *(const uint32_t*)p;
+    } else {
+      h = *(const uint16_t*)p;
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int i = 0; i < kPieces; i++) ((uint4*)p)[i] = q[i];
+    } else if constexpr (kBytes == 8) {
+      *(uint2*)p = d;
+    } else if constexpr (kBytes == 4) {
+      *(uint32_t*)p = w;
+    } else {
+      *(uint16_t*)p = h;
+    }
+  }
+  __device__ __forceinline__ float get(int i) const { return rw_widen(v[i]); }
+  __device__ __forceinline__ void set(int i, float f) { v[i] = rw_round<T>(f); }
+};
+
+// Whether a matrix of `elem`-byte elements can be read V elements at a time.
+inline bool rw_packs(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, size_t elem, int V) {
+  const size_t piece = std::min<size_t>(elem * V, 16);
+  return cols % V == 0 && (uintptr_t)p % piece == 0 && (rows <= 1 || ld * elem % piece == 0);
+}
+
 inline size_t rw_type_bytes(int type) { return type == RW_F32 ? 4 : 2; }
 
 // Calls f with a value of the element type `type` names.

@@ -813,6 +813,7 @@ struct DeviceScope {
 };
 
 constexpr uint64_t kMaxItems = (1ull << 31) - 1;
+constexpr uint64_t kMaxWidth = (1ull << 23) - 1;
 
 bool elem_type_ok(int32_t t) { return t == RW_F32 || t == RW_BF16 || t == RW_F16; }
 bool index_type_ok(int32_t t) { return t == RW_I32 || t == RW_I64; }
@@ -894,8 +895,9 @@ extern "C" int rw_embed_grad_workspace(rw_ctx* ctx, uint64_t n, uint64_t d, uint
                                        uint64_t* bytes) {
   if (!bytes) return fail(ctx, RW_ERR_ARG, "bytes is NULL");
   *bytes = 0;
-  if (n > kMaxItems || vocab > kMaxItems)
-    return fail(ctx, RW_ERR_ARG, "rw_embed_grad_workspace: n and vocab must be below 2^31");
+  if (n > kMaxItems || vocab > kMaxItems || d > kMaxWidth)
+    return fail(ctx, RW_ERR_ARG,
+                "rw_embed_grad_workspace: n and vocab must be below 2^31, d below 2^23");
   *bytes = embed_grad_workspace(n, d, vocab);
   return RW_OK;
 }
@@ -912,6 +914,7 @@ extern "C" int rw_embed_grad_device(rw_ctx* ctx, const void* d_grad, int32_t gra
         if (!elem_type_ok(grad_type) || !elem_type_ok(dtable_type)) return "unknown element type";
         if (!index_type_ok(id_type)) return "unknown id type";
         if (n > kMaxItems || vocab > kMaxItems) return "n and vocab must be below 2^31";
+        if (d > kMaxWidth) return "d must be below 2^23";
         RW_MATRIX(d_grad, n, d, ld_grad, elem_bytes(grad_type));
         RW_VECTOR(d_ids, n, index_bytes(id_type));
         RW_MATRIX(d_dtable, vocab, d, ld_dtable, elem_bytes(dtable_type));

@@ -66,6 +66,7 @@ CASES = [
     (embed_grad, dict(id_type=-1), "unknown id type"),
     (embed_grad, dict(n=1 << 31), "below 2^31"),
     (embed_grad, dict(vocab=1 << 31), "below 2^31"),
+    (embed_grad, dict(d=1 << 23, ld_grad=1 << 23, ld_dtable=1 << 23), "below 2^23"),
     (embed_grad, dict(grad=None), "d_grad is NULL"),
     (embed_grad, dict(ids=None), "d_ids is NULL"),
     (embed_grad, dict(dtable=None), "d_dtable is NULL"),
