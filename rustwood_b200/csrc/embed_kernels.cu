@@ -50,7 +50,7 @@ constexpr int kRadixBits = 9;
 constexpr int kRadix = 1 << kRadixBits;
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortRounds = 8;
+constexpr int kSortRounds = 4;
 constexpr int kSortTile = kSortThreads * kSortRounds;
 
 struct SortPass {
@@ -77,6 +77,7 @@ __device__ __forceinline__ uint32_t sort_digit(const SortPass& p, unsigned long 
 template <typename ID, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) k_token_count(SortPass p) {
   __shared__ uint32_t s_count[kRadix];
+  rw_dependent_start();
   for (int d = threadIdx.x; d < kRadix; d += kSortThreads) s_count[d] = 0;
   __syncthreads();
   const uint64_t lo = (uint64_t)blockIdx.x * p.part, hi = min(lo + p.part, p.n);
@@ -94,11 +95,18 @@ __global__ void __launch_bounds__(kSortThreads) k_token_scatter(SortPass p) {
   __shared__ uint32_t s_sum[kSortWarps];
   static_assert(kRadix == kSortThreads, "one thread a digit");
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  rw_dependent_start();
   uint32_t before = 0, total = 0;
-  for (uint32_t q = 0; q < p.parts; q++) {
-    const uint32_t c = p.counts[(uint64_t)q * kRadix + t];
-    before += q < blockIdx.x ? c : 0;
-    total += c;
+  for (uint32_t q0 = 0; q0 < p.parts; q0 += 16) {  // 16 loads in flight
+    uint32_t c[16];
+#pragma unroll
+    for (int u = 0; u < 16; u++)
+      c[u] = q0 + u < p.parts ? p.counts[(uint64_t)(q0 + u) * kRadix + t] : 0;
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+      before += q0 + u < blockIdx.x ? c[u] : 0;
+      total += c[u];
+    }
   }
   uint32_t incl = total;
 #pragma unroll
@@ -152,6 +160,37 @@ __global__ void __launch_bounds__(kSortThreads) k_token_scatter(SortPass p) {
   }
 }
 
+// Short inputs are sorted by counting instead, in one launch: a position's place is the
+// number of positions before it in the order (id, position). n * n comparisons: 2 us at
+// n = 512, and at kCountSort still less than the radix sort's launches.
+constexpr uint64_t kCountSort = 4096;
+constexpr int kCountThreads = 256;
+constexpr int kCountShare = 8;  // threads that share a position's comparisons
+
+template <typename ID>
+__global__ void __launch_bounds__(kCountThreads)
+    k_token_rank(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, unsigned long long* __restrict__ out) {
+  __shared__ uint32_t s_key[kCountSort];
+  for (uint32_t i = threadIdx.x; i < n; i += kCountThreads) {
+    const int64_t id = (int64_t)ids[i];
+    s_key[i] = id >= 0 && id < (int64_t)vocab ? (uint32_t)id : vocab;
+  }
+  __syncthreads();
+  const uint32_t t = blockIdx.x * kCountThreads + threadIdx.x, i = t / kCountShare, part = t % kCountShare;
+  const uint32_t key = i < n ? s_key[i] : 0;
+  uint32_t place = 0;
+  if (i < n) {
+#pragma unroll 4
+    for (uint32_t j = part; j < n; j += kCountShare) {
+      const uint32_t other = s_key[j];
+      place += other < key || (other == key && j < i);
+    }
+  }
+#pragma unroll
+  for (int o = kCountShare / 2; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+  if (i < n && part == 0) out[place] = (unsigned long long)key << 32 | i;
+}
+
 // The sums. The sorted positions are cut into chunks of equal length; a slot of `tx`
 // threads (V columns each) walks one chunk in order with its running sum in registers.
 // A run of equal ids inside one chunk is finished there; a run that crosses chunks leaves
@@ -195,6 +234,7 @@ __global__ void __launch_bounds__(kSumThreads)
                    float* __restrict__ partial) {
   const uint32_t slot = threadIdx.x / cp.tx, lane = threadIdx.x % cp.tx;
   TD* dtable = (TD*)a.dtable;
+  rw_dependent_start();
   if (blockIdx.x >= cp.sum_ctas) {  // zero the rows of this block that no id names
     __shared__ bool s_absent[kZeroRows];
     const uint64_t first = (uint64_t)(blockIdx.x - cp.sum_ctas) * kZeroRows;
@@ -288,6 +328,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t col = (uint64_t)blockIdx.y * kJoinCols + lane * 4;
   TD* dtable = (TD*)a.dtable;
+  rw_dependent_start();
 
   auto row_sum = [&](uint32_t first, uint32_t lo, uint32_t hi) {
     // partials lo..hi-1 of the run that starts in chunk `first`, in order
@@ -324,8 +365,12 @@ __global__ void __launch_bounds__(kJoinThreads)
       const uint64_t lo = c * cp.chunk, hi = lo + cp.chunk;
       const uint32_t key = key_of(pairs[hi - 1]);
       if (key < a.vocab && key_of(pairs[hi]) == key && (lo == 0 || key_of(pairs[lo - 1]) != key)) {
-        // the last chunk that begins with this id
+        // the last chunk that begins with this id: in growing steps, then by halving
         uint64_t in = c + 1, out = cp.chunks;
+        for (uint64_t step = 1; in + step < out; step *= 2) {
+          if (key_of(pairs[(in + step) * cp.chunk]) == key) in += step;
+          else out = in + step;
+        }
         while (out - in > 1) {
           const uint64_t mid = (in + out) / 2;
           if (key_of(pairs[mid * cp.chunk]) == key) in = mid;
@@ -451,9 +496,10 @@ struct GradPlan {
   uint64_t pairs0, pairs1, counts, partial, bytes;  // offsets
 };
 
-// Chunks: enough for about 16 CTAs an SM, so that the longest one does not decide the
-// time, but no shorter than 8 positions (the partial sums would be more than a quarter of
-// the traffic) and no more than 32768 (k_embed_join looks at each).
+// Chunks: enough for about 16 CTAs an SM where a row takes two warps or more, so that the
+// longest one does not decide the time; for narrower rows 4, whose slots are many and whose
+// runs then cross fewer chunks; no shorter than 8 positions (the partial sums would be more
+// than a quarter of the traffic) and no more than 32768 (k_embed_join looks at each).
 ChunkPlan chunk_plan(uint64_t n, uint64_t d, int V) {
   ChunkPlan c = {};
   c.dv = (d + V - 1) / V;
@@ -461,7 +507,7 @@ ChunkPlan chunk_plan(uint64_t n, uint64_t d, int V) {
   c.slots = kSumThreads / c.tx;
   c.col_blocks = (uint32_t)((c.dv + c.tx - 1) / c.tx);
   c.pitch = (d + 3) / 4 * 4;
-  const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * 16 * c.slots / c.col_blocks);
+  const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * (c.tx >= 64 ? 16 : 4) * c.slots / c.col_blocks);
   const uint64_t most = std::min<uint64_t>(want, 32768);
   c.chunk = (uint32_t)std::max<uint64_t>(8, (n + most - 1) / most);
   c.chunks = (uint32_t)((n + c.chunk - 1) / c.chunk);
@@ -516,6 +562,16 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   char* ws = (char*)workspace;
   unsigned long long* buf[2] = {(unsigned long long*)(ws + g.pairs0),
                                 (unsigned long long*)(ws + g.pairs1)};
+  const bool count = a.n <= kCountSort;
+  if (count) {
+    *nl += 1;
+    e = rw_with_index(a.id_type, [&](auto id) {
+      using ID = decltype(id);
+      const uint32_t blocks = (uint32_t)((a.n * kCountShare + kCountThreads - 1) / kCountThreads);
+      return rw_launch(k_token_rank<ID>, dim3(blocks), dim3(kCountThreads), 0, s, false,
+                       (const ID*)a.ids, (uint32_t)a.n, (uint32_t)a.vocab, buf[0]);
+    });
+  }
   SortPass p = {};
   p.ids = a.ids;
   p.counts = (uint32_t*)(ws + g.counts);
@@ -523,7 +579,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   p.part = g.part;
   p.vocab = a.vocab;
   p.parts = g.parts;
-  for (uint32_t i = 0; i < g.passes && e == cudaSuccess; i++) {
+  for (uint32_t i = 0; i < g.passes && !count && e == cudaSuccess; i++) {
     p.in = buf[(i + 1) & 1];
     p.out = buf[i & 1];
     p.shift = i * kRadixBits;
@@ -532,14 +588,14 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
       using ID = decltype(id);
       const dim3 grid(g.parts), block(kSortThreads);
       cudaError_t r = i == 0 ? rw_launch(k_token_count<ID, true>, grid, block, 0, s, false, p)
-                             : rw_launch(k_token_count<ID, false>, grid, block, 0, s, false, p);
+                             : rw_launch(k_token_count<ID, false>, grid, block, 0, s, true, p);
       if (r != cudaSuccess) return r;
-      return i == 0 ? rw_launch(k_token_scatter<ID, true>, grid, block, 0, s, false, p)
-                    : rw_launch(k_token_scatter<ID, false>, grid, block, 0, s, false, p);
+      return i == 0 ? rw_launch(k_token_scatter<ID, true>, grid, block, 0, s, true, p)
+                    : rw_launch(k_token_scatter<ID, false>, grid, block, 0, s, true, p);
     });
   }
   if (e != cudaSuccess) return e;
-  const unsigned long long* pairs = buf[(g.passes + 1) & 1];
+  const unsigned long long* pairs = count ? buf[0] : buf[(g.passes + 1) & 1];
   float* partial = (float*)(ws + g.partial);
   *nl += 2;
   ChunkPlan cp = {};
@@ -553,9 +609,9 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
       cp = chunk_plan(a.n, a.d, wide ? kV : 1);
       const uint64_t zero = a.accumulate ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
       const dim3 grid((uint32_t)(cp.sum_ctas + zero));
-      return wide ? rw_launch(k_embed_chunks<TG, TD, kV>, grid, dim3(kSumThreads), 0, s, false, a, cp,
+      return wide ? rw_launch(k_embed_chunks<TG, TD, kV>, grid, dim3(kSumThreads), 0, s, true, a, cp,
                               pairs, partial)
-                  : rw_launch(k_embed_chunks<TG, TD, 1>, grid, dim3(kSumThreads), 0, s, false, a, cp,
+                  : rw_launch(k_embed_chunks<TG, TD, 1>, grid, dim3(kSumThreads), 0, s, true, a, cp,
                               pairs, partial);
     });
   });
@@ -563,7 +619,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   const uint32_t cols = (uint32_t)((a.d + kJoinCols - 1) / kJoinCols);
   const uint32_t gx = std::max(1u, std::min(cp.chunks, (uint32_t)kSms * 4 / cols));
   return rw_with_type(a.dtable_type, [&](auto td) {
-    return rw_launch(k_embed_join<decltype(td)>, dim3(gx, cols), dim3(kJoinThreads), 0, s, false, a,
+    return rw_launch(k_embed_join<decltype(td)>, dim3(gx, cols), dim3(kJoinThreads), 0, s, true, a,
                      cp, pairs, (const float*)partial);
   });
 }

@@ -95,9 +95,16 @@ inline cudaError_t rw_with_index(int type, F f) {
   return cudaErrorInvalidValue;
 }
 
+// Programmatic dependent launch: a kernel launched as `dependent` (rw_launch) lets its
+// successor start, then waits until its predecessors' writes are visible.
+__device__ __forceinline__ void rw_dependent_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // A launch whose error is its own (an earlier, unrelated error of the thread stays where
 // it is). dependent: the launch may start while its predecessor on the stream runs; the
-// kernel waits for it (griddepcontrol.wait) before it touches global memory.
+// kernel calls rw_dependent_start() before it touches global memory.
 template <typename... KArgs, typename... Args>
 inline cudaError_t rw_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
                              bool dependent, Args... args) {
