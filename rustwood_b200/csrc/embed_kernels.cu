@@ -22,17 +22,45 @@ constexpr int kSms = 148;
 // =================================================================================
 // lookup
 
-template <typename TI, typename TO, typename ID>
-__global__ void __launch_bounds__(256) k_embed(EmbedLaunch a) {
+// A CTA takes `slots` rows at a time, `tx` threads a row, V columns a thread and kEmbedDepth
+// vectors in flight: one pass, each id read once per row of threads.
+constexpr int kEmbedThreads = 256;
+constexpr int kEmbedDepth = 4;
+
+struct EmbedPlan {
+  uint32_t tx, slots;
+  uint64_t dv;     // vectors a row
+  uint32_t split;  // CTAs that share a row's columns
+};
+
+template <typename TI, typename TO, typename ID, int V>
+__global__ void __launch_bounds__(kEmbedThreads) k_embed(EmbedLaunch a, EmbedPlan ep) {
+  const uint32_t slot = threadIdx.x / ep.tx, lane = threadIdx.x % ep.tx;
+  if (slot >= ep.slots) return;
   const TI* table = (const TI*)a.table;
   const ID* ids = (const ID*)a.ids;
-  TO* out = (TO*)a.out;
-  for (uint64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
+  const uint64_t step = (uint64_t)ep.tx * ep.split;
+  const uint64_t first = (uint64_t)(blockIdx.x % ep.split) * ep.tx + lane;
+  for (uint64_t i = (uint64_t)(blockIdx.x / ep.split) * ep.slots + slot; i < a.n;
+       i += (uint64_t)(gridDim.x / ep.split) * ep.slots) {
     const int64_t id = (int64_t)ids[i];
     const bool in = id >= 0 && (uint64_t)id < a.vocab;
     const TI* row = table + (in ? (uint64_t)id : 0) * a.ld_table;
-    for (uint64_t c = threadIdx.x; c < a.d; c += blockDim.x)
-      out[i * a.ld_out + c] = rw_round<TO>(in ? a.scale * rw_widen(row[c]) : 0.0f);
+    TO* out = (TO*)a.out + i * a.ld_out;
+    for (uint64_t c = first; c < ep.dv; c += step * kEmbedDepth) {
+      Pack<TI, V> v[kEmbedDepth];
+#pragma unroll
+      for (int u = 0; u < kEmbedDepth; u++)
+        if (in && c + u * step < ep.dv) v[u].load(row + (c + u * step) * V);
+#pragma unroll
+      for (int u = 0; u < kEmbedDepth; u++) {
+        if (c + u * step >= ep.dv) break;
+        Pack<TO, V> o;
+#pragma unroll
+        for (int k = 0; k < V; k++) o.set(k, in ? a.scale * v[u].get(k) : 0.0f);
+        o.store_streaming(out + (c + u * step) * V);
+      }
+    }
   }
 }
 
@@ -410,6 +438,107 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 }
 
+// Few, narrow table rows (a categorical column) need no sort: a slot of d threads keeps a
+// whole table of sums in shared memory, one column a thread, so no two threads share a sum
+// and the order is fixed (a sum of no rows stays at its start, -0); the CTA streams its part of grad once, in memory order. A sorted
+// walk reads rows of 132 bytes in category order instead, whose partly used sectors cost
+// twice the traffic.
+constexpr uint32_t kTableRows = 64;   // 256 threads x 64 rows x 4 bytes: 3 CTAs an SM
+constexpr uint32_t kTableCols = kSumThreads;
+constexpr int kTableDepth = 8;
+constexpr int kTableJoinThreads = 1024;
+
+struct TablePlan {
+  uint32_t slots, ctas;
+  uint64_t part;  // positions a CTA
+  size_t smem;
+};
+
+template <typename TG, typename ID>
+__global__ void __launch_bounds__(kSumThreads, 3)
+    k_embed_table(EmbedGradLaunch a, TablePlan tp, float* __restrict__ partial) {
+  extern __shared__ float s_table[];  // [slots][vocab + 1][d]
+  const uint32_t d = (uint32_t)a.d, vocab = (uint32_t)a.vocab, cells = vocab * d;
+  const uint32_t slot = threadIdx.x / d, col = threadIdx.x % d;
+  if (slot < tp.slots) {
+    float* table = s_table + slot * (cells + d) + col;
+    for (uint32_t v = 0; v <= vocab; v++) table[v * d] = -0.0f;
+    const uint64_t lo = (uint64_t)blockIdx.x * tp.part;
+    const uint32_t count = (uint32_t)min(tp.part, a.n - lo);  // lo < n
+    const ID* ids = (const ID*)a.ids + lo;
+    const TG* grad = (const TG*)a.grad + lo * a.ld_grad + col;
+    const uint32_t ld = (uint32_t)a.ld_grad;
+    // ids outside the table add to its last row, which is not read
+    auto cell = [&](ID id) -> float& {
+      return table[(id >= 0 && id < (ID)vocab ? (uint32_t)id : vocab) * d];
+    };
+    // a round of rows is added while the next round's loads are in flight
+    const uint32_t round = tp.slots * kTableDepth;
+    ID id[2][kTableDepth];
+    TG g[2][kTableDepth];
+    auto fetch = [&](int b, uint32_t from) {
+      const bool whole = from + (kTableDepth - 1) * tp.slots < count;
+#pragma unroll
+      for (int u = 0; u < kTableDepth; u++) {
+        const uint32_t at = from + u * tp.slots, i = whole ? at : min(at, count - 1);
+        id[b][u] = rw_load_here(ids + i);
+        g[b][u] = rw_load_here(grad + (uint64_t)i * ld);
+      }
+      if (!whole) {  // past the end: the last position again, for nobody
+#pragma unroll
+        for (int u = 0; u < kTableDepth; u++)
+          if (from + u * tp.slots >= count) id[b][u] = (ID)-1;
+      }
+    };
+    auto add = [&](int b) {
+#pragma unroll
+      for (int u = 0; u < kTableDepth; u++) cell(id[b][u]) += rw_widen(g[b][u]);
+    };
+    if (slot < count) fetch(0, slot);
+    for (uint32_t j = slot; j < count; j += 2 * round) {
+      if (j + round < count) fetch(1, j + round);
+      add(0);
+      if (j + round >= count) break;
+      if (j + 2 * round < count) fetch(0, j + 2 * round);
+      add(1);
+    }
+  }
+  __syncthreads();
+  for (uint32_t c = threadIdx.x; c < cells; c += kSumThreads) {
+    float s = s_table[c];
+    for (uint32_t k = 1; k < tp.slots; k++) s += s_table[k * (cells + d) + c];
+    partial[(uint64_t)blockIdx.x * cells + c] = s;
+  }
+}
+
+// dtable from the CTAs' tables: 32 cells a CTA, the tables shared by its warps in order.
+template <typename TD>
+__global__ void __launch_bounds__(kTableJoinThreads)
+    k_embed_table_join(EmbedGradLaunch a, uint32_t tables, const float* __restrict__ partial) {
+  constexpr int kWarps = kTableJoinThreads / 32;
+  __shared__ float s_part[kWarps][32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cells = (uint32_t)(a.vocab * a.d), c = blockIdx.x * 32 + lane;
+  rw_dependent_start();
+  const uint32_t per = (tables + kWarps - 1) / kWarps;
+  const uint32_t lo = min(tables, warp * per), hi = min(tables, lo + per);
+  float s = -0.0f;
+  if (c < cells) {
+#pragma unroll 8
+    for (uint32_t t = lo; t < hi; t++) s += partial[(uint64_t)t * cells + c];
+  }
+  s_part[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || c >= cells) return;
+  for (int w = 1; w < kWarps; w++) s += s_part[w][lane];
+  const uint32_t v = c / (uint32_t)a.d;
+  TD* p = (TD*)a.dtable + v * a.ld_dtable + (c - v * (uint32_t)a.d);
+  // -0 is the sum of no rows (or of -0 alone): nothing to add, whatever the scale is
+  const bool none = __float_as_uint(s) == 0x80000000u;
+  if (!a.accumulate) *p = rw_round<TD>(none ? 0.0f : s * a.scale);
+  else if (!none) *p = rw_round<TD>(rw_widen(*p) + s * a.scale);
+}
+
 template <typename TD>
 __global__ void __launch_bounds__(256) k_zero_rows(TD* p, uint64_t rows, uint64_t d, uint64_t ld) {
   for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x)
@@ -430,39 +559,78 @@ struct Words {
   uint32_t w[4];
 };
 
-__device__ __forceinline__ Words philox(uint64_t group, uint64_t sequence, uint64_t seed) {
+// The generator's ten round keys are the same for all: computed once on the host.
+struct PhiloxKeys {
+  uint32_t k0[10], k1[10];
+};
+
+__device__ __forceinline__ Words philox(uint64_t group, uint64_t sequence, const PhiloxKeys& k) {
   uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32);
   uint32_t c2 = (uint32_t)sequence, c3 = (uint32_t)(sequence >> 32);
-  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
   for (int r = 0; r < 10; r++) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k.k0[r];
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k.k1[r];
     c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return {{c0, c1, c2, c3}};
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_dropout(DropoutLaunch a) {
-  const uint64_t total = a.rows * a.cols, groups = (total + 7) / 8;
+__device__ __forceinline__ bool dropout_keep(const Words& w, int k, uint32_t limit) {
+  return (k & 1 ? w.w[k / 2] >> 16 : w.w[k / 2] & 0xffff) >= limit;
+}
+
+// One thread takes the 8 elements of a counter, two counters at a time so that two loads are
+// in flight while it computes. VEC: the matrices are contiguous and 16-byte aligned, so a
+// group is one or two 16-byte accesses; the last, partial one goes element by element.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_dropout(DropoutLaunch a, PhiloxKeys keys) {
+  const uint64_t total = a.rows * a.cols;
   const T* x = (const T*)a.x;
   T* y = (T*)a.y;
-  for (uint64_t g = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups;
-       g += (uint64_t)gridDim.x * blockDim.x) {
-    const Words w = philox(g, a.sequence, a.seed);
+  const uint64_t t = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const uint64_t threads = (uint64_t)gridDim.x * blockDim.x;
+  if (VEC) {
+    const uint64_t whole = total / 8;
+    for (uint64_t g = t; g < whole; g += 2 * threads) {
+      const bool two = g + threads < whole;
+      Pack<T, 8> v[2];
+      v[0].load(x + g * 8);
+      if (two) v[1].load(x + (g + threads) * 8);
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        if (b && !two) break;
+        const Words w = philox(g + b * threads, a.sequence, keys);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          v[b].set(k, dropout_keep(w, k, a.limit) ? v[b].get(k) * a.scale : 0.0f);
+        v[b].store(y + (g + b * threads) * 8);
+      }
+    }
+    if (t == 0 && whole * 8 < total) {
+      const Words w = philox(whole, a.sequence, keys);
+#pragma unroll
+      for (int k = 0; k < 7; k++) {
+        const uint64_t e = whole * 8 + k;
+        if (e < total) y[e] = rw_round<T>(dropout_keep(w, k, a.limit) ? rw_widen(x[e]) * a.scale : 0.0f);
+      }
+    }
+    return;
+  }
+  for (uint64_t g = t; g * 8 < total; g += threads) {
+    const Words w = philox(g, a.sequence, keys);
+    uint64_t r = g * 8 / a.cols, c = g * 8 - r * a.cols;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      const uint64_t e = g * 8 + k;
-      if (e >= total) break;
-      const uint64_t r = e / a.cols, c = e - r * a.cols;
-      const uint32_t half = k & 1 ? w.w[k / 2] >> 16 : w.w[k / 2] & 0xffff;
-      const float v = half >= a.limit ? rw_widen(x[r * a.ld_x + c]) * a.scale : 0.0f;
-      y[r * a.ld_y + c] = rw_round<T>(v);
+      if (g * 8 + k >= total) break;
+      y[r * a.ld_y + c] =
+          rw_round<T>(dropout_keep(w, k, a.limit) ? rw_widen(x[r * a.ld_x + c]) * a.scale : 0.0f);
+      if (++c == a.cols) {
+        c = 0;
+        r++;
+      }
     }
   }
 }
@@ -479,8 +647,27 @@ cudaError_t launch_embed(const EmbedLaunch& a, cudaStream_t s, int* nl) {
   return rw_with_type(a.table_type, [&](auto ti) {
     return rw_with_type(a.out_type, [&](auto to) {
       return rw_with_index(a.id_type, [&](auto id) {
-        return rw_launch(k_embed<decltype(ti), decltype(to), decltype(id)>, dim3(grid_of(a.n, 8)),
-                         dim3(256), 0, s, false, a);
+        using TI = decltype(ti);
+        using TO = decltype(to);
+        using ID = decltype(id);
+        constexpr int kV = 16 / sizeof(TI);
+        const bool wide = rw_packs(a.table, a.vocab, a.d, a.ld_table, sizeof(TI), kV) &&
+                          rw_packs(a.out, a.n, a.d, a.ld_out, sizeof(TO), kV);
+        EmbedPlan ep;
+        ep.dv = wide ? a.d / kV : a.d;
+        // many rows: kEmbedDepth vectors a thread where a row has a warp's worth of them
+        uint64_t tx = std::min<uint64_t>(ep.dv, kEmbedThreads);
+        if (a.n >= 8 * kSms && ep.dv >= 32 * kEmbedDepth)
+          tx = std::min<uint64_t>((ep.dv / kEmbedDepth + 31) / 32 * 32, kEmbedThreads);
+        ep.tx = (uint32_t)tx;
+        ep.slots = kEmbedThreads / ep.tx;
+        // few rows: a row's columns over several CTAs, one vector a thread
+        const uint64_t groups = (a.n + ep.slots - 1) / ep.slots;
+        const uint64_t most = (ep.dv + ep.tx - 1) / ep.tx;
+        ep.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 2 * kSms / groups));
+        const dim3 grid(grid_of(groups, 8) * ep.split);
+        return wide ? rw_launch(k_embed<TI, TO, ID, kV>, grid, dim3(kEmbedThreads), 0, s, false, a, ep)
+                    : rw_launch(k_embed<TI, TO, ID, 1>, grid, dim3(kEmbedThreads), 0, s, false, a, ep);
       });
     });
   });
@@ -515,6 +702,21 @@ ChunkPlan chunk_plan(uint64_t n, uint64_t d, int V) {
   return c;
 }
 
+bool table_fits(uint64_t d, uint64_t vocab) { return d <= kTableCols && vocab <= kTableRows; }
+
+TablePlan table_plan(uint64_t n, uint64_t d, uint64_t vocab) {
+  TablePlan t;
+  t.slots = (uint32_t)(kTableCols / d);
+  t.smem = (size_t)t.slots * (vocab + 1) * d * 4;
+  const uint64_t per_sm = std::max<uint64_t>(1, std::min<uint64_t>(3, (200u << 10) / (t.smem + 1024)));
+  // two full rounds of loads a slot at least
+  const uint64_t least = (uint64_t)t.slots * kTableDepth * 2;
+  const uint64_t ctas = std::max<uint64_t>(1, std::min<uint64_t>(kSms * per_sm, n / least));
+  t.part = (n + ctas - 1) / ctas;
+  t.ctas = (uint32_t)((n + t.part - 1) / t.part);
+  return t;
+}
+
 GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
   GradPlan g;
   const uint64_t tiles = (n + kSortTile - 1) / kSortTile;
@@ -525,6 +727,11 @@ GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
   while (bits < 32 && vocab >> bits) bits++;  // keys 0..vocab
   g.passes = (bits + kRadixBits - 1) / kRadixBits;
   uint64_t at = 0;
+  if (table_fits(d, vocab)) {
+    g.pairs0 = g.pairs1 = g.counts = g.partial = 0;
+    g.bytes = (uint64_t)table_plan(n, d, vocab).ctas * vocab * d * 4;
+    return g;
+  }
   auto take = [&](uint64_t bytes) {
     const uint64_t o = at;
     at += (bytes + 255) / 256 * 256;
@@ -560,6 +767,25 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   }
   const GradPlan g = grad_plan(a.n, a.d, a.vocab);
   char* ws = (char*)workspace;
+  if (table_fits(a.d, a.vocab)) {
+    // rows further than 2^32 elements apart are out of any memory's range
+    const TablePlan t = table_plan(a.n, a.d, a.vocab);
+    *nl += 2;
+    e = rw_with_type(a.grad_type, [&](auto tg) {
+      return rw_with_index(a.id_type, [&](auto id) {
+        auto* k = k_embed_table<decltype(tg), decltype(id)>;
+        cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)((kTableRows + 1) * kTableCols * 4));
+        if (r != cudaSuccess) return r;
+        return rw_launch(k, dim3(t.ctas), dim3(kSumThreads), t.smem, s, false, a, t, (float*)ws);
+      });
+    });
+    if (e != cudaSuccess) return e;
+    return rw_with_type(a.dtable_type, [&](auto td) {
+      return rw_launch(k_embed_table_join<decltype(td)>, dim3((uint32_t)((a.vocab * a.d + 31) / 32)),
+                       dim3(kTableJoinThreads), 0, s, true, a, t.ctas, (const float*)ws);
+    });
+  }
   unsigned long long* buf[2] = {(unsigned long long*)(ws + g.pairs0),
                                 (unsigned long long*)(ws + g.pairs1)};
   const bool count = a.n <= kCountSort;
@@ -628,8 +854,17 @@ cudaError_t launch_dropout(const DropoutLaunch& a, cudaStream_t s, int* nl) {
   if (a.rows == 0 || a.cols == 0) return cudaSuccess;
   *nl += 1;
   const uint64_t groups = (a.rows * a.cols + 7) / 8;
+  PhiloxKeys keys;
+  for (uint32_t r = 0; r < 10; r++) {
+    keys.k0[r] = (uint32_t)a.seed + r * 0x9E3779B9u;
+    keys.k1[r] = (uint32_t)(a.seed >> 32) + r * 0xBB67AE85u;
+  }
+  const bool flat = a.rows == 1 || (a.ld_x == a.cols && a.ld_y == a.cols);
+  const bool vec = flat && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.y % 16 == 0;
   return rw_with_type(a.type, [&](auto t) {
-    return rw_launch(k_dropout<decltype(t)>, dim3(grid_of((groups + 255) / 256, 8)), dim3(256), 0, s,
-                     false, a);
+    using T = decltype(t);
+    const dim3 grid(grid_of((groups + 255) / 256, 8)), block(256);
+    return vec ? rw_launch(k_dropout<T, true>, grid, block, 0, s, false, a, keys)
+               : rw_launch(k_dropout<T, false>, grid, block, 0, s, false, a, keys);
   });
 }
