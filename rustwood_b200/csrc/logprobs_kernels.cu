@@ -16,7 +16,7 @@
 // It takes m and log_sum rather than lse: lse in 32 bits cannot hold log_sum beside a large
 // m (the finite lowest value used as a mask).
 #include <cuda_runtime.h>
-#include <math_constants.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -26,8 +26,9 @@
 
 namespace {
 
-constexpr int kRowThreads = 256;
-constexpr float kLowest = -1e30f;  // where d is cut: e^d is 0 there, and 0 * d stays 0
+constexpr float kLowest = -1e30f;  // where differences are cut: e^d is 0 there, and 0 * d stays 0
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = INFINITY;
 
 // The larger of two values, NaN if either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -35,92 +36,516 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
-// Orders margins (NaN above +inf, -0 equal to +0), then lower indices first.
-__device__ __forceinline__ unsigned long long rank_key(float x, uint32_t index) {
+// An order of the margins as whole numbers above 0 (NaN above +inf, -0 equal to +0), and with
+// the index below it: larger margins first, lower indices first among equal ones.
+__device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
-  const uint32_t o = x != x ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (unsigned long long)o << 32 | (0xffffffffu - index);
+  return x != x ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float margin_of(uint32_t order) {
+  return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+using Key = unsigned long long;
+__device__ __forceinline__ Key key_of(uint32_t order, uint32_t index) {
+  return (Key)order << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t index_of(Key k) { return 0xffffffffu - (uint32_t)k; }
+
+// A running softmax: the largest margin so far, s = sum e^{scale (x - m)} and
+// t = sum e^{scale (x - m)} (x - m). c = scale * log2(e).
+struct Sums {
+  float m = -kInf, s = 0.0f, t = 0.0f;
+};
+// Restates the sums relative to a larger maximum (not -inf).
+__device__ __forceinline__ void raise(Sums& a, float m, float c) {
+  const float d = max_nan(a.m - m, kLowest), f = exp2_fast(d * c);
+  a.t = f * (a.t + d * a.s);
+  a.s *= f;
+  a.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+  const float m = max_nan(a.m, b.m);
+  if (m == -kInf) return a;
+  raise(a, m, c);
+  raise(b, m, c);
+  a.s += b.s;
+  a.t += b.t;
+  return a;
+}
+__device__ __forceinline__ Sums shuffle_xor(const Sums& a, int o) {
+  Sums b;
+  b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+  b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+  b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
+  return b;
 }
 
-template <typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, V* s_tmp, F f) {
+// What the outputs of a row need of its sums.
+struct RowEnd {
+  float base, log_sum;  // base: the maximum, 0 in a row of -inf alone
+};
+__device__ __forceinline__ RowEnd row_end(const Sums& a) {
+  const bool dead = a.m == -kInf;
+  return {dead ? 0.0f : a.m, dead ? 0.0f : logf(a.s)};
+}
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobsLaunch& a, uint64_t i, const Sums& r, const RowEnd& e) {
+  if (a.row_max) a.row_max[i] = r.m;
+  if (a.log_sum) a.log_sum[i] = e.log_sum;
+  if (a.lse) a.lse[i] = a.scale * r.m + e.log_sum;
+  if (a.entropy) a.entropy[i] = r.m == -kInf ? 0.0f : e.log_sum - a.scale * (r.t / r.s);
+  if (a.logp) {
+    const int64_t c = a.target_type == RW_I64 ? ((const int64_t*)a.targets)[i] : ((const int32_t*)a.targets)[i];
+    float v = 0.0f;
+    if (c >= 0 && (uint64_t)c < a.classes)
+      v = (rw_widen(((const T*)a.x)[i * a.ld_x + c]) - e.base) * a.scale - e.log_sum;
+    a.logp[i] = v;
+  }
+}
+__device__ __forceinline__ void write_top(const LogprobsLaunch& a, uint64_t i, uint32_t place, Key k, const RowEnd& e) {
+  if (a.top_index) a.top_index[i * a.top_k + place] = index_of(k);
+  if (a.top_logp)
+    a.top_logp[i * a.top_k + place] = (margin_of((uint32_t)(k >> 32)) - e.base) * a.scale - e.log_sum;
+}
+
+// =================================================================================
+// Few classes: L lanes a row, at most E margins a lane, all in registers.
+
+constexpr int kGroupThreads = 256;
+constexpr int kGroupCand = 128;  // candidates for a row's top places that a warp keeps
+
+template <typename T, int L, int E>
+__global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a) {
+  __shared__ Key s_cand[L == 32 ? kGroupThreads / 32 : 1][L == 32 ? kGroupCand : 1];
+  const uint32_t lane = threadIdx.x % L, classes = (uint32_t)a.classes;
+  const float c = a.scale * kLog2e;
+  constexpr uint32_t kRows = kGroupThreads / L;  // rows of a CTA at a time
+  for (uint64_t base = (uint64_t)blockIdx.x * kRows; base < a.n; base += (uint64_t)gridDim.x * kRows) {
+    const uint64_t i = base + threadIdx.x / L;
+    const bool real = i < a.n;
+    const T* x = (const T*)a.x + (real ? i : a.n - 1) * a.ld_x;
+    float v[E];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s_tmp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = s_tmp[0];
-  for (int w = 1; w < kRowThreads / 32; w++) v = f(v, s_tmp[w]);
-  return v;
-}
-
-template <typename T, typename ID>
-__global__ void __launch_bounds__(kRowThreads) k_logprobs(LogprobsLaunch a) {
-  __shared__ float s_f[kRowThreads / 32];
-  __shared__ unsigned long long s_k[kRowThreads / 32];
-  for (uint64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-    const T* x = (const T*)a.x + i * a.ld_x;
-    float m = -CUDART_INF_F;
-    for (uint64_t j = threadIdx.x; j < a.classes; j += kRowThreads) m = max_nan(m, rw_widen(x[j]));
-    m = block_reduce(m, s_f, max_nan);
-    const bool dead = m == -CUDART_INF_F;
-    const float base = dead ? 0.0f : m;
-    float s = 0.0f, t = 0.0f;
-    for (uint64_t j = threadIdx.x; j < a.classes; j += kRowThreads) {
-      const float d = max_nan((rw_widen(x[j]) - base) * a.scale, kLowest);
-      const float e = expf(d);
-      s += e;
-      t += e * d;
+    for (int e = 0; e < E; e++) {
+      const uint32_t j = lane + e * L;
+      v[e] = j < classes ? rw_widen(x[j]) : -kInf;
     }
-    auto add = [](float p, float q) { return p + q; };
-    s = block_reduce(s, s_f, add);
-    t = block_reduce(t, s_f, add);
-    const float log_sum = dead ? 0.0f : logf(s);
-    if (threadIdx.x == 0) {
-      if (a.row_max) a.row_max[i] = m;
-      if (a.log_sum) a.log_sum[i] = log_sum;
-      if (a.lse) a.lse[i] = a.scale * m + log_sum;
-      if (a.entropy) a.entropy[i] = dead ? 0.0f : log_sum - t / s;
-      if (a.logp) {
-        const int64_t c = (int64_t)((const ID*)a.targets)[i];
-        const bool in = c >= 0 && (uint64_t)c < a.classes;
-        a.logp[i] = in ? (rw_widen(x[c]) - base) * a.scale - log_sum : 0.0f;
+    Sums r;
+#pragma unroll
+    for (int e = 0; e < E; e++) r.m = max_nan(r.m, v[e]);
+    const float own = r.m;
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) r.m = max_nan(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
+    if (r.m != -kInf) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float d = max_nan(v[e] - r.m, kLowest), p = exp2_fast(d * c);
+        r.s += p;
+        r.t += p * d;
       }
     }
-    unsigned long long last = ~0ull;
-    for (uint32_t k = 0; k < a.top_k; k++) {
-      unsigned long long best = 0;
-      for (uint64_t j = threadIdx.x; j < a.classes; j += kRowThreads) {
-        const unsigned long long key = rank_key(rw_widen(x[j]), (uint32_t)j);
-        if ((k == 0 || key < last) && key > best) best = key;
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+      r.t += __shfl_xor_sync(0xffffffffu, r.t, o);
+    }
+    const RowEnd end = row_end(r);
+    if (real && lane == 0) write_row<T>(a, i, r, end);
+    if (a.top_k == 0) continue;
+    if constexpr (L == 32) {
+      // The top_k-th largest of the lanes' maxima is a bound: top_k margins at least reach it.
+      // Those that do (the bound's own included) are ranked by counting. Too many only if
+      // many are equal or a lane holds many of the largest: then place by place, below.
+      const uint32_t mine = order_of(own);
+      uint32_t above = 0;
+#pragma unroll
+      for (int o = 0; o < 32; o++) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, o);
+        above += other > mine || (other == mine && o < (int)lane);
       }
-      best = last = block_reduce(best, s_k, [](unsigned long long p, unsigned long long q) {
-        return p > q ? p : q;
-      });
-      if (threadIdx.x == 0) {
-        const uint32_t j = 0xffffffffu - (uint32_t)best;
-        if (a.top_index) a.top_index[i * a.top_k + k] = j;
-        if (a.top_logp) a.top_logp[i * a.top_k + k] = (rw_widen(x[j]) - base) * a.scale - log_sum;
+      const uint32_t who = __ballot_sync(0xffffffffu, above == a.top_k - 1);
+      const uint32_t bound = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
+      Key* cand = s_cand[threadIdx.x / 32];
+      uint32_t count = 0;
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const uint32_t o = order_of(v[e]);
+        const bool in = o >= bound && lane + e * 32 < classes;
+        const uint32_t hits = __ballot_sync(0xffffffffu, in);
+        const uint32_t at = count + __popc(hits & ((1u << lane) - 1));
+        if (in && at < kGroupCand) cand[at] = key_of(o, lane + e * 32);
+        count += __popc(hits);
+      }
+      __syncwarp();
+      if (count <= kGroupCand) {
+        for (uint32_t q = lane; q < count; q += 32) {
+          const Key k = cand[q];
+          uint32_t place = 0;
+          for (uint32_t w = 0; w < count; w++) place += cand[w] > k;
+          if (real && place < a.top_k) write_top(a, i, place, k, end);
+        }
+        continue;
       }
     }
-    __syncthreads();
+    Key last = ~0ull;
+    for (uint32_t place = 0; place < a.top_k; place++) {
+      Key best = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const uint32_t j = lane + e * L;
+        const Key k = j < classes ? key_of(order_of(v[e]), j) : 0;
+        if (k < last && k > best) best = k;
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      last = best;
+      if (real && lane == 0) write_top(a, i, place, best, end);
+    }
   }
 }
 
+// =================================================================================
+// Many classes: a CTA a row, or a part of one.
+
+constexpr int kRowThreads = 512;
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowDepth = 4;       // vectors in flight a thread
+constexpr uint32_t kGroups = 128;  // groups of threads whose maxima bound the top places
+constexpr uint32_t kCand = 1024;   // candidates for the top places that a CTA keeps
+constexpr uint32_t kMaxParts = 64;
+
+// Where a row's sums and top keys are left when it is split: [row][part].
+struct SplitRow {
+  uint32_t parts;
+  uint64_t part;  // classes a part
+  Sums* sums;
+  Key* keys;      // [row][part][top_k], descending
+};
+
+// Consecutive margins as 16-byte vectors with a ragged head and tail.
+template <typename T>
+struct Span {
+  static constexpr int kV = 16 / sizeof(T);
+  const T* x;
+  uint32_t n, head, vecs;
+  __device__ __forceinline__ Span(const T* p, uint32_t count) : x(p), n(count) {
+    const uint32_t off = (uint32_t)((uintptr_t)p & 15) / sizeof(T);
+    head = min(n, off ? kV - off : 0u);
+    vecs = (n - head) / kV;
+  }
+  __device__ __forceinline__ uint32_t ragged() const { return n - vecs * kV; }
+  // the position of ragged element r
+  __device__ __forceinline__ uint32_t ragged_at(uint32_t r) const { return r < head ? r : vecs * kV + r; }
+  __device__ __forceinline__ const T* vec(uint32_t v) const { return x + head + (size_t)v * kV; }
+};
+
+// The largest of V elements, NaN if one is.
+template <int V>
+__device__ __forceinline__ float pack_max(const Pack<float, V>& p) {
+  float m = p.v[0];
+#pragma unroll
+  for (int k = 1; k < V; k++) m = max_nan(m, p.v[k]);
+  return m;
+}
+template <typename T, typename T2, int V>
+__device__ __forceinline__ T2 pair_max(const Pack<T, V>& p) {
+  const T2* w = reinterpret_cast<const T2*>(p.v);
+  T2 m = w[0];
+#pragma unroll
+  for (int k = 1; k < V / 2; k++) m = __hmax2_nan(m, w[k]);
+  return m;
+}
+template <int V>
+__device__ __forceinline__ float pack_max(const Pack<__nv_bfloat16, V>& p) {
+  const __nv_bfloat162 m = pair_max<__nv_bfloat16, __nv_bfloat162, V>(p);
+  return max_nan(__low2float(m), __high2float(m));
+}
+template <int V>
+__device__ __forceinline__ float pack_max(const Pack<__half, V>& p) {
+  const __half2 m = pair_max<__half, __half2, V>(p);
+  return max_nan(__low2float(m), __high2float(m));
+}
+
+struct TopSpace {
+  uint32_t order[kRowThreads];  // each thread's largest
+  uint32_t group[kGroups];
+  Key cand[kCand];
+  uint32_t warp[kRowWarps];
+  Key warp_key[kRowWarps];
+  uint32_t count, bound;
+};
+
+// The top_k places among the span's margins, in order, given every thread's largest margin;
+// emit(place, key) is called once a place. All threads of the CTA call it.
+template <typename T, typename Emit>
+__device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32_t top_k, TopSpace& s, Emit emit) {
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  constexpr int kV = Span<T>::kV;
+  const uint32_t mine = order_of(own);
+  __syncthreads();
+  s.order[t] = mine;
+  if (t == 0) s.count = 0;
+  __syncthreads();
+  // A bound that top_k margins at least reach: the top_k-th largest of the groups' maxima.
+  // The threads of a group are far apart, so neighbours in a row fall into different groups.
+  if (t < kGroups) {
+    uint32_t g = s.order[t];
+#pragma unroll
+    for (uint32_t q = t + kGroups; q < kRowThreads; q += kGroups) g = max(g, s.order[q]);
+    s.group[t] = g;
+  }
+  __syncthreads();
+  if (t < kGroups) {
+    const uint32_t g = s.group[t];
+    uint32_t above = 0;
+#pragma unroll 8
+    for (uint32_t q = 0; q < kGroups; q++) {
+      const uint32_t o = s.group[q];
+      above += o > g || (o == g && q < t);
+    }
+    if (above == top_k - 1) s.bound = g;
+  }
+  __syncthreads();
+  const uint32_t bound = s.bound;
+  // Collects the margins whose order is at least `from` (only threads that have one look).
+  auto collect = [&](uint32_t from) {
+    if (mine < from) return;
+    auto offer = [&](float x, uint32_t j) {
+      const uint32_t o = order_of(x);
+      if (o < from) return;
+      const uint32_t at = atomicAdd(&s.count, 1u);
+      if (at < kCand) s.cand[at] = key_of(o, offset + j);
+    };
+    for (uint32_t v = t; v < sp.vecs; v += kRowThreads) {
+      Pack<T, kV> p;
+      p.load(sp.vec(v));
+      if (order_of(pack_max(p)) < from) continue;
+#pragma unroll
+      for (int k = 0; k < kV; k++) offer(p.get(k), sp.head + v * kV + k);
+    }
+    if (t < sp.ragged()) offer(rw_widen(sp.x[sp.ragged_at(t)]), sp.ragged_at(t));
+  };
+  collect(bound);
+  __syncthreads();
+  uint32_t count = s.count;
+  uint32_t ties = 0;  // places that go to margins equal to the bound, in index order
+  if (count > kCand) {
+    // Many margins equal to the bound (a mask, a constant row): only those above it are
+    // candidates, and the first of the equal ones follow.
+    __syncthreads();
+    if (t == 0) s.count = 0;
+    __syncthreads();
+    if (bound != 0xffffffffu) collect(bound + 1);
+    __syncthreads();
+    count = s.count;
+    ties = count < top_k ? top_k - count : 0;
+  }
+  if (count <= kCand) {
+    for (uint32_t q = t; q < count; q += kRowThreads) {
+      const Key k = s.cand[q];
+      uint32_t place = 0;
+      for (uint32_t w = 0; w < count; w++) place += s.cand[w] > k;
+      if (place < top_k) emit(place, k);
+    }
+    uint32_t place = top_k - ties;  // the next place for an equal one
+    for (uint32_t j0 = 0; place < top_k && j0 < sp.n; j0 += kRowThreads) {
+      const uint32_t j = j0 + t;
+      const bool in = j < sp.n && order_of(rw_widen(sp.x[j])) == bound;
+      const uint32_t hits = __ballot_sync(0xffffffffu, in);
+      __syncthreads();
+      if (lane == 0) s.warp[warp] = __popc(hits);
+      __syncthreads();
+      uint32_t before = 0, all = 0;
+      for (int w = 0; w < kRowWarps; w++) {
+        before += w < (int)warp ? s.warp[w] : 0;
+        all += s.warp[w];
+      }
+      const uint32_t at = place + before + __popc(hits & ((1u << lane) - 1));
+      if (in && at < top_k) emit(at, key_of(bound, offset + j));
+      place += all;
+    }
+    return;
+  }
+  // The largest margins are more than the candidates' space and lie in few groups: place by
+  // place over the whole span.
+  Key last = ~0ull;
+  for (uint32_t place = 0; place < top_k; place++) {
+    Key best = 0;
+    for (uint32_t j = t; j < sp.n; j += kRowThreads) {
+      const Key k = key_of(order_of(rw_widen(sp.x[j])), offset + j);
+      if (k < last && k > best) best = k;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    __syncthreads();
+    if (lane == 0) s.warp_key[warp] = best;
+    __syncthreads();
+    for (int w = 0; w < kRowWarps; w++) best = max(best, s.warp_key[w]);
+    last = best;
+    if (t == 0) emit(place, best);
+  }
+}
+
+// One pass over a row (or part): 16-byte vectors, kRowDepth in flight; a thread restates its
+// sums only when a block of kRowDepth vectors holds a new maximum. ENT: with the entropy's sum.
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kRowThreads, 3) k_logprobs_row(LogprobsLaunch a, SplitRow sr) {
+  __shared__ TopSpace s_top;
+  __shared__ Sums s_sums[kRowWarps];
+  constexpr int kV = Span<T>::kV;
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint64_t i = blockIdx.x / sr.parts;
+  const uint32_t part = blockIdx.x % sr.parts;
+  const uint64_t lo = part * sr.part, hi = min(lo + sr.part, a.classes);
+  const Span<T> sp((const T*)a.x + i * a.ld_x + lo, (uint32_t)(hi - lo));
+  const float c = a.scale * kLog2e;
+
+  Sums r;
+  float s2 = 0.0f, t2 = 0.0f;  // a second pair of sums, relative to the same maximum
+  auto add = [&](float x, float& s, float& w) {
+    const float d = x - r.m, e = exp2_fast(d * c);
+    s += e;
+    if (ENT) w = __fmaf_rn(e, max_nan(d, kLowest), w);
+  };
+  auto absorb = [&](const Pack<T, kV>* p, int count) {  // count: a constant after unrolling
+    float m = pack_max(p[0]);
+#pragma unroll
+    for (int u = 1; u < kRowDepth; u++)
+      if (u < count) m = max_nan(m, pack_max(p[u]));
+    if (!(m <= r.m)) {
+      r.s += s2;
+      r.t += t2;
+      s2 = t2 = 0.0f;
+      raise(r, max_nan(r.m, m), c);
+    }
+    if (r.m == -kInf) return;
+#pragma unroll
+    for (int u = 0; u < kRowDepth; u++) {
+      if (u >= count) break;
+#pragma unroll
+      for (int k = 0; k < kV; k += 2) {
+        add(p[u].get(k), r.s, r.t);
+        add(p[u].get(k + 1), s2, t2);
+      }
+    }
+  };
+  uint32_t v = t;
+  for (; v + (kRowDepth - 1) * kRowThreads < sp.vecs; v += kRowDepth * kRowThreads) {
+    Pack<T, kV> p[kRowDepth];
+#pragma unroll
+    for (int u = 0; u < kRowDepth; u++) p[u].load(sp.vec(v + u * kRowThreads));
+    absorb(p, kRowDepth);
+  }
+  for (; v < sp.vecs; v += kRowThreads) {
+    Pack<T, kV> p;
+    p.load(sp.vec(v));
+    absorb(&p, 1);
+  }
+  r.s += s2;
+  r.t += t2;
+  if (t < sp.ragged()) {
+    Sums one;
+    one.m = rw_widen(sp.x[sp.ragged_at(t)]);
+    one.s = one.m == -kInf ? 0.0f : 1.0f;
+    r = join(r, one, c);
+  }
+  const float own = r.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
+  if (lane == 0) s_sums[warp] = r;
+  __syncthreads();
+  r = s_sums[lane % kRowWarps];
+#pragma unroll
+  for (int o = kRowWarps / 2; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
+  if (sr.parts == 1) {
+    const RowEnd end = row_end(r);
+    if (t == 0) write_row<T>(a, i, r, end);
+    if (a.top_k)
+      top_places(sp, 0u, own, a.top_k, s_top, [&](uint32_t place, Key k) { write_top(a, i, place, k, end); });
+  } else {
+    if (t == 0) sr.sums[blockIdx.x] = r;
+    if (a.top_k) {
+      Key* keys = sr.keys + (uint64_t)blockIdx.x * a.top_k;
+      // a part may have fewer classes than places
+      if (t < a.top_k) keys[t] = 0;
+      const uint32_t places = min(a.top_k, sp.n);
+      top_places(sp, (uint32_t)lo, own, places, s_top, [&](uint32_t place, Key k) { keys[place] = k; });
+    }
+  }
+}
+
+// Joins a split row: the parts' sums, and the top places of their sorted lists (a list whose
+// head is below the top_k-th largest head has none).
+template <typename T>
+__global__ void __launch_bounds__(256) k_logprobs_join(LogprobsLaunch a, SplitRow sr) {
+  __shared__ Key s_head[kMaxParts];
+  __shared__ Key s_cand[kMaxTop * kMaxTop + kMaxTop];
+  __shared__ uint32_t s_count;
+  __shared__ Key s_bound;
+  const uint32_t t = threadIdx.x, lane = t & 31;
+  const uint64_t i = blockIdx.x;
+  const float c = a.scale * kLog2e;
+  rw_dependent_start();
+  const Sums* sums = sr.sums + i * sr.parts;
+  Sums r;
+  if (lane < sr.parts) r = sums[lane];
+  if (lane + 32 < sr.parts) r = join(r, sums[lane + 32], c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
+  const RowEnd end = row_end(r);
+  if (t == 0) write_row<T>(a, i, r, end);
+  if (a.top_k == 0) return;
+  const Key* keys = sr.keys + i * sr.parts * a.top_k;
+  if (t < sr.parts) s_head[t] = keys[(uint64_t)t * a.top_k];
+  if (t == 0) {
+    s_count = 0;
+    s_bound = 1;  // fewer lists than places: every key counts
+  }
+  __syncthreads();
+  if (sr.parts >= a.top_k && t < sr.parts) {
+    uint32_t above = 0;
+    for (uint32_t q = 0; q < sr.parts; q++) above += s_head[q] > s_head[t];
+    if (above == a.top_k - 1) s_bound = s_head[t];
+  }
+  __syncthreads();
+  const Key bound = s_bound;
+  // at most top_k lists have a head at the bound or above
+  for (uint32_t q = t; q < sr.parts * a.top_k; q += 256) {
+    if (s_head[q / a.top_k] < bound) continue;
+    const Key k = keys[q];
+    if (k >= bound) s_cand[atomicAdd(&s_count, 1u)] = k;
+  }
+  __syncthreads();
+  const uint32_t count = s_count;
+  for (uint32_t q = t; q < count; q += 256) {
+    const Key k = s_cand[q];
+    uint32_t place = 0;
+    for (uint32_t w = 0; w < count; w++) place += s_cand[w] > k;
+    if (place < a.top_k) write_top(a, i, place, k, end);
+  }
+}
+
+constexpr int kGradThreads = 256;
 template <typename T, typename ID>
-__global__ void __launch_bounds__(kRowThreads) k_logprobs_grad(LogprobsGradLaunch a) {
+__global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaunch a) {
   for (uint64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
     const T* x = (const T*)a.x + i * a.ld_x;
     T* dx = (T*)a.dx + i * a.ld_dx;
     const float m = a.row_max[i], log_sum = a.log_sum[i];
-    const bool dead = m == -CUDART_INF_F;
+    const bool dead = m == -kInf;
     int64_t c = a.targets ? (int64_t)((const ID*)a.targets)[i] : -1;
     if (c < 0 || (uint64_t)c >= a.classes) c = -1;
     const float g = c >= 0 ? a.grad_logp[i] : 0.0f;
     const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f;
     const float h = a.grad_entropy ? a.entropy[i] : 0.0f;
-    for (uint64_t j = threadIdx.x; j < a.classes; j += kRowThreads) {
+    for (uint64_t j = threadIdx.x; j < a.classes; j += kGradThreads) {
       const float lp = max_nan((rw_widen(x[j]) - m) * a.scale - log_sum, kLowest);
       const float p = expf(lp);
       float v = (int64_t)j == c ? g : 0.0f;
@@ -134,18 +559,59 @@ uint32_t grid_of(uint64_t blocks, uint32_t per_sm) {
   return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(blocks, 148ull * per_sm));
 }
 
+constexpr uint64_t kFewClasses = 1024;
+
+// Parts a row: with fewer rows than four CTAs an SM, enough parts to make that many, of 4096
+// classes at least (a vector a thread).
+SplitRow split_of(uint64_t n, uint64_t classes) {
+  SplitRow r = {1, classes, nullptr, nullptr};
+  if (classes <= kFewClasses || n == 0 || n >= 148 * 4) return r;
+  const uint64_t want = (148 * 4 + n - 1) / n;
+  const uint64_t parts = std::min<uint64_t>({want, kMaxParts, std::max<uint64_t>(1, classes / 4096)});
+  r.part = ((classes + parts - 1) / parts + 7) / 8 * 8;
+  r.parts = (uint32_t)((classes + r.part - 1) / r.part);
+  return r;
+}
+
 }  // namespace
 
-uint64_t logprobs_workspace(uint64_t, uint64_t, int, uint32_t) { return 0; }
+uint64_t logprobs_workspace(uint64_t n, uint64_t classes, int, uint32_t top_k) {
+  const SplitRow r = split_of(n, classes);
+  if (r.parts == 1) return 0;
+  const uint64_t cells = n * r.parts;
+  return (cells * sizeof(Sums) + 255) / 256 * 256 + cells * top_k * sizeof(Key);
+}
 
-cudaError_t launch_logprobs(const LogprobsLaunch& a, void*, cudaStream_t s, int* nl) {
+cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream_t s, int* nl) {
   if (a.n == 0) return cudaSuccess;
   *nl += 1;
-  return rw_with_type(a.type, [&](auto t) {
-    return rw_with_index(a.target_type, [&](auto id) {
-      return rw_launch(k_logprobs<decltype(t), decltype(id)>, dim3(grid_of(a.n, 8)),
-                       dim3(kRowThreads), 0, s, false, a);
+  if (a.classes <= kFewClasses)
+    return rw_with_type(a.type, [&](auto t) {
+      using T = decltype(t);
+      auto go = [&](auto* k, uint64_t lanes) {
+        const uint64_t rows = kGroupThreads / lanes;
+        return rw_launch(k, dim3(grid_of((a.n + rows - 1) / rows, 32)), dim3(kGroupThreads), 0, s, false, a);
+      };
+      if (a.classes <= 8) return go(k_logprobs_few<T, 1, 8>, 1);
+      if (a.classes <= 32) return go(k_logprobs_few<T, 4, 8>, 4);
+      if (a.classes <= 128) return go(k_logprobs_few<T, 8, 16>, 8);
+      if (a.classes <= 256) return go(k_logprobs_few<T, 32, 8>, 32);
+      if (a.classes <= 512) return go(k_logprobs_few<T, 32, 16>, 32);
+      return go(k_logprobs_few<T, 32, 32>, 32);
     });
+  SplitRow r = split_of(a.n, a.classes);
+  const uint64_t cells = a.n * r.parts;
+  if (cells > 0x7fffffffull) return cudaErrorInvalidValue;
+  r.sums = (Sums*)workspace;
+  r.keys = (Key*)((char*)workspace + (cells * sizeof(Sums) + 255) / 256 * 256);
+  return rw_with_type(a.type, [&](auto t) {
+    using T = decltype(t);
+    const dim3 grid((uint32_t)cells), block(kRowThreads);
+    cudaError_t e = a.entropy ? rw_launch(k_logprobs_row<T, true>, grid, block, 0, s, false, a, r)
+                              : rw_launch(k_logprobs_row<T, false>, grid, block, 0, s, false, a, r);
+    if (e != cudaSuccess || r.parts == 1) return e;
+    *nl += 1;
+    return rw_launch(k_logprobs_join<T>, dim3((uint32_t)a.n), dim3(256), 0, s, true, a, r);
   });
 }
 
@@ -155,7 +621,7 @@ cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, in
   return rw_with_type(a.type, [&](auto t) {
     return rw_with_index(a.target_type, [&](auto id) {
       return rw_launch(k_logprobs_grad<decltype(t), decltype(id)>, dim3(grid_of(a.n, 8)),
-                       dim3(kRowThreads), 0, s, false, a);
+                       dim3(kGradThreads), 0, s, false, a);
     });
   });
 }
