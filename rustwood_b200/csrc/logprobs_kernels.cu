@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
 // =================================================================================
 // Many classes: a CTA a row, or a part of one.
 
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
 constexpr uint32_t kGroups = 128;  // groups of threads whose maxima bound the top places
@@ -245,6 +245,49 @@ struct Span {
   __device__ __forceinline__ uint32_t ragged_at(uint32_t r) const { return r < head ? r : vecs * kV + r; }
   __device__ __forceinline__ const T* vec(uint32_t v) const { return x + head + (size_t)v * kV; }
 };
+
+// Two f32 values in a 64-bit register: one instruction adds or multiplies both.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two_of(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(Two v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// Elements 2 q and 2 q + 1 of a pack; CUT: not below kLowest.
+template <bool CUT, int V>
+__device__ __forceinline__ Two pair_of(const Pack<float, V>& p, int q) {
+  const float a = p.v[2 * q], b = p.v[2 * q + 1];
+  return CUT ? two_of(max_nan(a, kLowest), max_nan(b, kLowest)) : two_of(a, b);
+}
+template <bool CUT, int V>
+__device__ __forceinline__ Two pair_of(const Pack<__nv_bfloat16, V>& p, int q) {
+  __nv_bfloat162 w = reinterpret_cast<const __nv_bfloat162*>(p.v)[q];
+  if (CUT) w = __hmax2_nan(w, __float2bfloat162_rn(kLowest));
+  const uint32_t b = *reinterpret_cast<uint32_t*>(&w);
+  return two_of(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
+}
+template <bool CUT, int V>
+__device__ __forceinline__ Two pair_of(const Pack<__half, V>& p, int q) {
+  // the lowest f16 above -inf is far above kLowest: only -inf is cut, to that
+  __half2 w = reinterpret_cast<const __half2*>(p.v)[q];
+  const float2 f = __half22float2(w);
+  return CUT ? two_of(max_nan(f.x, kLowest), max_nan(f.y, kLowest)) : two_of(f.x, f.y);
+}
 
 // The largest of V elements, NaN if one is.
 template <int V>
@@ -314,21 +357,24 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
   }
   __syncthreads();
   const uint32_t bound = s.bound;
-  // Collects the margins whose order is at least `from` (only threads that have one look).
+  // Collects the margins whose order is at least `from`: a warp reads again, with all its
+  // lanes, the vectors of each thread that has one.
   auto collect = [&](uint32_t from) {
-    if (mine < from) return;
     auto offer = [&](float x, uint32_t j) {
       const uint32_t o = order_of(x);
       if (o < from) return;
       const uint32_t at = atomicAdd(&s.count, 1u);
       if (at < kCand) s.cand[at] = key_of(o, offset + j);
     };
-    for (uint32_t v = t; v < sp.vecs; v += kRowThreads) {
-      Pack<T, kV> p;
-      p.load(sp.vec(v));
-      if (order_of(pack_max(p)) < from) continue;
+    for (uint32_t who = __ballot_sync(0xffffffffu, mine >= from); who; who &= who - 1) {
+      const uint32_t first = warp * 32 + __ffs(who) - 1;
+      for (uint32_t v = first + lane * kRowThreads; v < sp.vecs; v += 32 * kRowThreads) {
+        Pack<T, kV> p;
+        p.load(sp.vec(v));
+        if (order_of(pack_max(p)) < from) continue;
 #pragma unroll
-      for (int k = 0; k < kV; k++) offer(p.get(k), sp.head + v * kV + k);
+        for (int k = 0; k < kV; k++) offer(p.get(k), sp.head + v * kV + k);
+      }
     }
     if (t < sp.ragged()) offer(rw_widen(sp.x[sp.ragged_at(t)]), sp.ragged_at(t));
   };
@@ -393,63 +439,135 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
   }
 }
 
-// One pass over a row (or part): 16-byte vectors, kRowDepth in flight; a thread restates its
-// sums only when a block of kRowDepth vectors holds a new maximum. ENT: with the entropy's sum.
+// The whole CTA's maximum, and its sum of v.x and v.y, in a fixed order.
+__device__ __forceinline__ float cta_max(float m, float* s_tmp) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) s_tmp[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = s_tmp[0];
+#pragma unroll
+  for (int w = 1; w < kRowWarps; w++) m = max_nan(m, s_tmp[w]);
+  return m;
+}
+__device__ __forceinline__ float2 cta_sum(float2 v, float2* s_tmp) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  if ((threadIdx.x & 31) == 0) s_tmp[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s_tmp[0];
+#pragma unroll
+  for (int w = 1; w < kRowWarps; w++) {
+    v.x += s_tmp[w].x;
+    v.y += s_tmp[w].y;
+  }
+  return v;
+}
+
+// One pass over a row (or part): 16-byte vectors, kRowDepth in flight, exponents as one
+// fused multiply-add e = x * c - mc with mc = round(m * c); the rounding of mc is known
+// exactly and taken out of the sums at the end. A thread restates its sums only when a block
+// of kRowDepth vectors holds a new maximum.
+//
+// x * c must not overflow: margins below kLowest count as kLowest, and blocks whose maximum
+// so far is not above it are left out. That is exact where the row's maximum is above
+// kLowest; where it is not (a row masked with the type's lowest value), and for scales
+// outside [kScaleLow, kScaleHigh], the sums are taken again as e^{scale (x - m)}.
+// ENT: with the entropy's sum.
+constexpr float kScaleLow = 1e-6f, kScaleHigh = 1e6f;
+
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kRowThreads, 3) k_logprobs_row(LogprobsLaunch a, SplitRow sr) {
+__global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch a, SplitRow sr) {
   __shared__ TopSpace s_top;
-  __shared__ Sums s_sums[kRowWarps];
+  __shared__ float s_max[kRowWarps];
+  __shared__ float2 s_sum[kRowWarps];
   constexpr int kV = Span<T>::kV;
-  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint32_t t = threadIdx.x;
   const uint64_t i = blockIdx.x / sr.parts;
   const uint32_t part = blockIdx.x % sr.parts;
   const uint64_t lo = part * sr.part, hi = min(lo + sr.part, a.classes);
   const Span<T> sp((const T*)a.x + i * a.ld_x + lo, (uint32_t)(hi - lo));
   const float c = a.scale * kLog2e;
 
-  Sums r;
-  float s2 = 0.0f, t2 = 0.0f;  // a second pair of sums, relative to the same maximum
-  auto add = [&](float x, float& s, float& w) {
-    const float d = x - r.m, e = exp2_fast(d * c);
-    s += e;
-    if (ENT) w = __fmaf_rn(e, max_nan(d, kLowest), w);
-  };
+  float m = -kInf, mc = 0.0f;
+  Two s = 0, w = 0, c2 = two_of(c, c), base = 0;  // base: -mc twice
   auto absorb = [&](const Pack<T, kV>* p, int count) {  // count: a constant after unrolling
-    float m = pack_max(p[0]);
+    float top = pack_max(p[0]);
 #pragma unroll
     for (int u = 1; u < kRowDepth; u++)
-      if (u < count) m = max_nan(m, pack_max(p[u]));
-    if (!(m <= r.m)) {
-      r.s += s2;
-      r.t += t2;
-      s2 = t2 = 0.0f;
-      raise(r, max_nan(r.m, m), c);
+      if (u < count) top = max_nan(top, pack_max(p[u]));
+    if (!(top <= m)) {
+      top = max_nan(top, m);
+      const float next = top * c;
+      if (m > kLowest) {
+        const float d = mc - next, f = exp2_fast(max_nan(d, kLowest));
+        const Two f2 = two_of(f, f), zero = 0;
+        if (ENT) w = fma2(f2, fma2(two_of(d, d), s, w), zero);
+        s = fma2(f2, s, zero);
+      }
+      m = top;
+      mc = next;
+      base = two_of(-next, -next);
     }
-    if (r.m == -kInf) return;
+    if (m <= kLowest) return;
 #pragma unroll
     for (int u = 0; u < kRowDepth; u++) {
       if (u >= count) break;
 #pragma unroll
-      for (int k = 0; k < kV; k += 2) {
-        add(p[u].get(k), r.s, r.t);
-        add(p[u].get(k + 1), s2, t2);
+      for (int q = 0; q < kV / 2; q++) {
+        const Two d = fma2(pair_of<ENT>(p[u], q), c2, base);
+        const float2 df = both(d);
+        const Two e = two_of(exp2_fast(df.x), exp2_fast(df.y));
+        s = add2(s, e);
+        if (ENT) w = fma2(e, d, w);
       }
     }
   };
+  // a block is summed while the next one's loads are in flight
+  constexpr uint32_t kBlock = kRowDepth * kRowThreads;
   uint32_t v = t;
-  for (; v + (kRowDepth - 1) * kRowThreads < sp.vecs; v += kRowDepth * kRowThreads) {
-    Pack<T, kV> p[kRowDepth];
+  auto fetch = [&](Pack<T, kV>* p, uint32_t from) {
 #pragma unroll
-    for (int u = 0; u < kRowDepth; u++) p[u].load(sp.vec(v + u * kRowThreads));
-    absorb(p, kRowDepth);
+    for (int u = 0; u < kRowDepth; u++) p[u].load(sp.vec(from + u * kRowThreads));
+  };
+  auto whole = [&](uint32_t from) { return from + (kRowDepth - 1) * kRowThreads < sp.vecs; };
+  if (whole(v)) {
+    Pack<T, kV> p[2][kRowDepth];
+    fetch(p[0], v);
+    for (;;) {
+      v += kBlock;
+      if (!whole(v)) {
+        absorb(p[0], kRowDepth);
+        break;
+      }
+      fetch(p[1], v);
+      absorb(p[0], kRowDepth);
+      v += kBlock;
+      if (!whole(v)) {
+        absorb(p[1], kRowDepth);
+        break;
+      }
+      fetch(p[0], v);
+      absorb(p[1], kRowDepth);
+    }
   }
   for (; v < sp.vecs; v += kRowThreads) {
     Pack<T, kV> p;
     p.load(sp.vec(v));
     absorb(&p, 1);
   }
-  r.s += s2;
-  r.t += t2;
+  Sums r;
+  r.m = m;
+  if (!(m <= kLowest)) {
+    // the sums are those of e^{scale (x - m)} times 2^off
+    const float off = __fmaf_rn(m, c, -mc), f = exp2_fast(-off);
+    const float2 sf = both(s), wf = both(w);
+    r.s = (sf.x + sf.y) * f;
+    r.t = ENT ? ((wf.x + wf.y) - off * (sf.x + sf.y)) * f / c : 0.0f;
+  }
   if (t < sp.ragged()) {
     Sums one;
     one.m = rw_widen(sp.x[sp.ragged_at(t)]);
@@ -457,13 +575,21 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_logprobs_row(LogprobsLaunch 
     r = join(r, one, c);
   }
   const float own = r.m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
-  if (lane == 0) s_sums[warp] = r;
-  __syncthreads();
-  r = s_sums[lane % kRowWarps];
-#pragma unroll
-  for (int o = kRowWarps / 2; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
+  const float all = cta_max(own, s_max);
+  if (all != -kInf) {
+    if ((all <= kLowest) || !(a.scale >= kScaleLow && a.scale <= kScaleHigh)) {
+      r.s = r.t = 0.0f;
+      for (uint32_t j = t; j < sp.n; j += kRowThreads) {
+        const float d = max_nan(rw_widen(sp.x[j]) - all, kLowest), e = exp2_fast(d * c);
+        r.s += e;
+        r.t += e * d;
+      }
+    } else {
+      raise(r, all, c);
+    }
+  }
+  const float2 sums = cta_sum(make_float2(r.s, r.t), s_sum);
+  r = {all, sums.x, sums.y};
   if (sr.parts == 1) {
     const RowEnd end = row_end(r);
     if (t == 0) write_row<T>(a, i, r, end);
