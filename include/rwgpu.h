@@ -359,8 +359,8 @@ int rw_logprobs_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n, u
 /* The gradient of sum_i (grad_logp[i] * logp[i] + grad_entropy[i] * entropy[i]) with
  * respect to the margins, from rw_logprobs_device's row_max, log_sum and (with
  * d_grad_entropy) entropy. d_targets with d_grad_logp, and d_grad_entropy, are each
- * nullable. A target outside 0..classes-1 contributes nothing; a row whose row_max is -inf
- * has a gradient of zeros. dx has the margins' type and may be x (with the same stride). */
+ * nullable. A target outside 0..classes-1 contributes nothing; a row whose row_max is -inf,
+ * or whose grad_logp and grad_entropy are both zero or absent, has a gradient of zeros. dx has the margins' type and may be x (with the same stride). */
 int rw_logprobs_grad_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n,
                             uint64_t classes, uint64_t ld_x, float scale, const void* d_targets,
                             int32_t target_type, const float* d_row_max, const float* d_log_sum,

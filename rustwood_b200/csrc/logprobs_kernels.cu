@@ -219,6 +219,7 @@ constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
 constexpr uint32_t kGroups = 128;  // groups of threads whose maxima bound the top places
 constexpr uint32_t kCand = 1024;   // candidates for the top places that a CTA keeps
+constexpr uint32_t kRare = 2 * kMaxTop;  // threads that reach the bound, if few margins equal it
 constexpr uint32_t kMaxParts = 64;
 
 // Where a row's sums and top keys are left when it is split: [row][part].
@@ -378,11 +379,12 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
     }
     if (t < sp.ragged()) offer(rw_widen(sp.x[sp.ragged_at(t)]), sp.ragged_at(t));
   };
-  collect(bound);
+  const bool rare = __syncthreads_count(mine >= bound) <= (int)kRare;
+  if (rare) collect(bound);
   __syncthreads();
   uint32_t count = s.count;
   uint32_t ties = 0;  // places that go to margins equal to the bound, in index order
-  if (count > kCand) {
+  if (!rare || count > kCand) {
     // Many margins equal to the bound (a mask, a constant row): only those above it are
     // candidates, and the first of the equal ones follow.
     __syncthreads();
@@ -658,26 +660,157 @@ __global__ void __launch_bounds__(256) k_logprobs_join(LogprobsLaunch a, SplitRo
   }
 }
 
+// =================================================================================
+// The gradient: elementwise, as dx = hit - 2^d (A + B d) with d = x * c - K and the row's
+// constants K = m c + log_sum log2(e), A, B and (at the target) hit. K is rounded to f32 and
+// what the rounding dropped is a factor of A and B, so large margins lose nothing.
+
 constexpr int kGradThreads = 256;
-template <typename T, typename ID>
-__global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaunch a) {
-  for (uint64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-    const T* x = (const T*)a.x + i * a.ld_x;
-    T* dx = (T*)a.dx + i * a.ld_dx;
-    const float m = a.row_max[i], log_sum = a.log_sum[i];
-    const bool dead = m == -kInf;
-    int64_t c = a.targets ? (int64_t)((const ID*)a.targets)[i] : -1;
-    if (c < 0 || (uint64_t)c >= a.classes) c = -1;
-    const float g = c >= 0 ? a.grad_logp[i] : 0.0f;
-    const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f;
-    const float h = a.grad_entropy ? a.entropy[i] : 0.0f;
-    for (uint64_t j = threadIdx.x; j < a.classes; j += kGradThreads) {
-      const float lp = max_nan((rw_widen(x[j]) - m) * a.scale - log_sum, kLowest);
-      const float p = expf(lp);
-      float v = (int64_t)j == c ? g : 0.0f;
-      v -= p * (g + e * (lp + h));
-      dx[j] = rw_round<T>(dead ? 0.0f : v * a.scale);
+constexpr int kGradDepth = 4;
+
+struct RowGrad {
+  float k, a, b, hit;
+  int32_t target;  // -1: none
+  int32_t kind;    // 0: zeros, 1: by the constants, 2: by the formula
+};
+
+__device__ __forceinline__ RowGrad row_grad(const LogprobsGradLaunch& a, uint64_t i) {
+  RowGrad r = {0.0f, 0.0f, 0.0f, 0.0f, -1, 0};
+  const float m = a.row_max[i];
+  if (m == -kInf) return r;
+  float g = 0.0f;
+  if (a.targets) {
+    const int64_t t = a.target_type == RW_I64 ? ((const int64_t*)a.targets)[i] : ((const int32_t*)a.targets)[i];
+    if (t >= 0 && (uint64_t)t < a.classes) {
+      r.target = (int32_t)t;
+      g = a.grad_logp[i];
     }
+  }
+  const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f;
+  if (g == 0.0f && e == 0.0f) return r;
+  // the constants would overflow below kLowest and for scales far from 1
+  if (m <= kLowest || !(a.scale >= kScaleLow && a.scale <= kScaleHigh)) {
+    r.kind = 2;
+    return r;
+  }
+  const double k = (double)m * (double)(a.scale * kLog2e) + (double)a.log_sum[i] * 1.4426950408889634;
+  r.k = (float)k;
+  const float rest = (float)(k - (double)r.k), f = exp2_fast(-rest) * a.scale;
+  const float h = a.grad_entropy ? a.entropy[i] : 0.0f;
+  constexpr float kLn2 = 0.6931471805599453f;
+  r.a = f * (g + e * (h - rest * kLn2));
+  r.b = f * e * kLn2;
+  r.hit = g * a.scale;
+  r.kind = 1;
+  return r;
+}
+// One element by the formula.
+__device__ __forceinline__ float grad_of(const LogprobsGradLaunch& a, uint64_t i, float x, bool hit, bool in) {
+  const float lp = max_nan((x - a.row_max[i]) * a.scale - a.log_sum[i], kLowest);
+  const float g = in ? a.grad_logp[i] : 0.0f;
+  const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f, h = a.grad_entropy ? a.entropy[i] : 0.0f;
+  return ((hit ? g : 0.0f) - exp2_fast(lp * kLog2e) * (g + e * (lp + h))) * a.scale;
+}
+__device__ __forceinline__ float grad_element(const LogprobsGradLaunch& a, uint64_t i, const RowGrad& r, float c,
+                                              float x, uint32_t j) {
+  const bool hit = (int32_t)j == r.target;
+  if (r.kind == 2) return grad_of(a, i, x, hit, r.target >= 0);
+  const float d = __fmaf_rn(max_nan(x, kLowest), c, -r.k);
+  const float v = -exp2_fast(d) * __fmaf_rn(r.b, d, r.a);
+  return hit ? v + r.hit : v;
+}
+
+// Many classes: a CTA takes kGradThreads * kGradDepth vectors of one row. x and dx lie the
+// same distance from a 16-byte boundary (VEC), else it goes element by element.
+template <typename T, bool VEC, bool ENT>
+__global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaunch a, uint32_t chunks) {
+  constexpr int kV = Span<T>::kV;
+  const uint64_t i = blockIdx.x / chunks;
+  const uint32_t chunk = blockIdx.x % chunks, t = threadIdx.x;
+  const Span<T> sp((const T*)a.x + i * a.ld_x, (uint32_t)a.classes);
+  T* dx = (T*)a.dx + i * a.ld_dx;
+  const RowGrad r = row_grad(a, i);
+  const float c = a.scale * kLog2e;
+  if (!VEC) {
+    constexpr uint32_t kPer = kGradThreads * kGradDepth * kV;
+    const uint32_t end = min((uint32_t)a.classes, (chunk + 1) * kPer);
+    for (uint32_t j = chunk * kPer + t; j < end; j += kGradThreads)
+      dx[j] = rw_round<T>(r.kind ? grad_element(a, i, r, c, rw_widen(sp.x[j]), j) : 0.0f);
+    return;
+  }
+  T* out = dx + sp.head;
+  const uint32_t v0 = chunk * (kGradThreads * kGradDepth) + t;
+  Pack<T, kV> p[kGradDepth];
+  if (r.kind) {
+#pragma unroll
+    for (int u = 0; u < kGradDepth; u++)
+      if (v0 + u * kGradThreads < sp.vecs) p[u].load(sp.vec(v0 + u * kGradThreads));
+  }
+  if (chunk == 0 && t < sp.ragged()) {
+    const uint32_t j = sp.ragged_at(t);
+    dx[j] = rw_round<T>(r.kind ? grad_element(a, i, r, c, rw_widen(sp.x[j]), j) : 0.0f);
+  }
+  // the target's vector, none: beyond the last
+  const uint32_t hit = r.target >= (int32_t)sp.head ? ((uint32_t)r.target - sp.head) / kV : 0xffffffffu;
+  const Two c2 = two_of(c, c), k2 = two_of(-r.k, -r.k), a2 = two_of(-r.a, -r.a), b2 = two_of(-r.b, -r.b);
+#pragma unroll
+  for (int u = 0; u < kGradDepth; u++) {
+    const uint32_t v = v0 + u * kGradThreads;
+    if (v >= sp.vecs) break;
+    if (r.kind == 1 && v != hit) {
+#pragma unroll
+      for (int q = 0; q < kV / 2; q++) {
+        const Two d = fma2(pair_of<ENT>(p[u], q), c2, k2);
+        const float2 df = both(d), w = ENT ? both(fma2(b2, d, a2)) : make_float2(-r.a, -r.a);
+        p[u].set(2 * q, exp2_fast(df.x) * w.x);
+        p[u].set(2 * q + 1, exp2_fast(df.y) * w.y);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kV; k++)
+        p[u].set(k, r.kind ? grad_element(a, i, r, c, p[u].get(k), sp.head + v * kV + k) : 0.0f);
+    }
+    p[u].store(out + (size_t)v * kV);
+  }
+}
+
+// Few classes: a CTA takes `rows` whole rows, their constants in shared memory. VEC: the
+// matrices are contiguous and aligned, so the rows are one run of 16-byte vectors whose
+// elements may lie in different rows.
+constexpr uint32_t kGradRows = 1024;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGradLaunch a, uint32_t rows) {
+  __shared__ RowGrad s_row[kGradRows];
+  constexpr int kV = VEC ? 16 / (int)sizeof(T) : 1;
+  const uint64_t first = (uint64_t)blockIdx.x * rows;
+  const uint32_t count = (uint32_t)min((uint64_t)rows, a.n - first), classes = (uint32_t)a.classes;
+  for (uint32_t k = threadIdx.x; k < count; k += kGradThreads) s_row[k] = row_grad(a, first + k);
+  __syncthreads();
+  const float c = a.scale * kLog2e;
+  const uint32_t total = count * classes;
+  const T* x = (const T*)a.x + first * a.ld_x;
+  T* dx = (T*)a.dx + first * a.ld_dx;
+  for (uint32_t j0 = threadIdx.x * kV; j0 < total; j0 += kGradThreads * kV) {
+    uint32_t row = j0 / classes, j = j0 - row * classes;
+    RowGrad r = s_row[row];
+    Pack<T, kV> p;
+    const bool all = VEC && j0 + kV <= total;
+    if (all) p.load(x + j0);
+#pragma unroll
+    for (int k = 0; k < kV; k++) {
+      if (!all && j0 + k >= total) break;
+      const size_t from = VEC ? j0 + k : row * a.ld_x + j, to = VEC ? j0 + k : row * a.ld_dx + j;
+      const float in = all ? p.get(k) : rw_widen(x[from]);
+      const float v = r.kind ? grad_element(a, first + row, r, c, in, j) : 0.0f;
+      if (all) p.set(k, v);
+      else dx[to] = rw_round<T>(v);
+      if (kV > 1 && ++j == classes && j0 + k + 1 < total) {
+        j = 0;
+        r = s_row[++row];
+      }
+    }
+    if (all) p.store(dx + j0);
   }
 }
 
@@ -741,13 +874,34 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
   });
 }
 
+// Up to this many classes rows share CTAs.
+constexpr uint64_t kGradFew = 2048;
+
 cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, int* nl) {
   if (a.n == 0 || a.classes == 0) return cudaSuccess;
   *nl += 1;
   return rw_with_type(a.type, [&](auto t) {
-    return rw_with_index(a.target_type, [&](auto id) {
-      return rw_launch(k_logprobs_grad<decltype(t), decltype(id)>, dim3(grid_of(a.n, 8)),
-                       dim3(kGradThreads), 0, s, false, a);
-    });
+    using T = decltype(t);
+    constexpr uint64_t kV = 16 / sizeof(T);
+    const dim3 block(kGradThreads);
+    const uintptr_t x = (uintptr_t)a.x, dx = (uintptr_t)a.dx;
+    const bool one = a.n == 1;
+    if (a.classes <= kGradFew) {
+      const bool vec = x % 16 == 0 && dx % 16 == 0 && (one || (a.ld_x == a.classes && a.ld_dx == a.classes));
+      // about kGradDepth vectors a thread, whole vectors in whole rows
+      uint64_t rows = kGradThreads * kGradDepth * kV / a.classes;
+      rows = std::min<uint64_t>(std::max<uint64_t>(rows, 1) + kV - 1, kGradRows) / kV * kV;
+      const uint64_t ctas = (a.n + rows - 1) / rows;
+      if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
+      return vec ? rw_launch(k_logprobs_grad_few<T, true>, dim3((uint32_t)ctas), block, 0, s, false, a, (uint32_t)rows)
+                 : rw_launch(k_logprobs_grad_few<T, false>, dim3((uint32_t)ctas), block, 0, s, false, a, (uint32_t)rows);
+    }
+    const bool vec = x % 16 == dx % 16 && (one || (a.ld_x * sizeof(T)) % 16 == (a.ld_dx * sizeof(T)) % 16);
+    const uint64_t per = kGradThreads * kGradDepth * kV, chunks = (a.classes + per - 1) / per;
+    if (a.n * chunks > 0x7fffffffull) return cudaErrorInvalidValue;
+    const dim3 grid((uint32_t)(a.n * chunks));
+    if (!vec) return rw_launch(k_logprobs_grad<T, false, true>, grid, block, 0, s, false, a, (uint32_t)chunks);
+    return a.grad_entropy ? rw_launch(k_logprobs_grad<T, true, true>, grid, block, 0, s, false, a, (uint32_t)chunks)
+                          : rw_launch(k_logprobs_grad<T, true, false>, grid, block, 0, s, false, a, (uint32_t)chunks);
   });
 }
