@@ -140,7 +140,8 @@ def test_bad_arguments_are_refused(call, change, message):
 def test_workspace_queries():
     b = C.c_uint64(7)
     assert N.lib.rw_embed_grad_workspace(None, 0, 8, 10, C.byref(b)) == 0 and b.value == 0
-    assert N.lib.rw_embed_grad_workspace(None, 1000, 8, 10, C.byref(b)) == 0 and b.value >= 16000
+    for vocab in (10, 1000):  # summed in tables, and by sorting
+        assert N.lib.rw_embed_grad_workspace(None, 10000, 8, vocab, C.byref(b)) == 0 and b.value > 0
     assert N.lib.rw_embed_grad_workspace(None, 1 << 31, 8, 10, C.byref(b)) == -1 and b.value == 0
     assert N.lib.rw_embed_grad_workspace(None, 1, 1, 1, None) == -1
     for bad in ((5, 2, 100), (F32, 33, 100), (F32, 2, 1 << 31)):
