@@ -188,6 +188,27 @@ __global__ void __launch_bounds__(kSortThreads) k_token_scatter(SortPass p) {
   }
 }
 
+// Rows of zeros, as bytes: `unit`-byte stores (16, or the element's size) by `threads` threads.
+struct ZeroRows {
+  char* p;
+  uint64_t rows, row_units, pitch;  // pitch in bytes
+  uint32_t unit;
+};
+__device__ __forceinline__ void zero_units(const ZeroRows& z, uint64_t t, uint64_t threads) {
+  auto put = [&](char* p) {
+    if (z.unit == 16) __stcs((uint4*)p, make_uint4(0, 0, 0, 0));
+    else if (z.unit == 4) *(uint32_t*)p = 0;
+    else *(uint16_t*)p = 0;
+  };
+  if (z.rows == 1) {
+    for (uint64_t c = t; c < z.row_units; c += threads) put(z.p + c * z.unit);
+    return;
+  }
+  const uint64_t warp = t / 32, warps = threads / 32;  // a warp a row
+  for (uint64_t r = warp; r < z.rows; r += warps)
+    for (uint64_t c = t % 32; c < z.row_units; c += 32) put(z.p + r * z.pitch + c * z.unit);
+}
+
 // Short inputs are sorted by counting instead, in one launch: a position's place is the
 // number of positions before it in the order (id, position). n * n comparisons: 2 us at
 // n = 512, and at kCountSort still less than the radix sort's launches.
@@ -195,10 +216,17 @@ constexpr uint64_t kCountSort = 4096;
 constexpr int kCountThreads = 256;
 constexpr int kCountShare = 8;  // threads that share a position's comparisons
 
+// The CTAs from `blocks` on zero the table meanwhile, when there is one to zero.
 template <typename ID>
 __global__ void __launch_bounds__(kCountThreads)
-    k_token_rank(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, unsigned long long* __restrict__ out) {
+    k_token_rank(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, unsigned long long* __restrict__ out,
+                 uint32_t blocks, ZeroRows z) {
   __shared__ uint32_t s_key[kCountSort];
+  if (blockIdx.x >= blocks) {
+    zero_units(z, (uint64_t)(blockIdx.x - blocks) * kCountThreads + threadIdx.x,
+               (uint64_t)(gridDim.x - blocks) * kCountThreads);
+    return;
+  }
   for (uint32_t i = threadIdx.x; i < n; i += kCountThreads) {
     const int64_t id = (int64_t)ids[i];
     s_key[i] = id >= 0 && id < (int64_t)vocab ? (uint32_t)id : vocab;
@@ -539,10 +567,8 @@ __global__ void __launch_bounds__(kTableJoinThreads)
   else if (!none) *p = rw_round<TD>(rw_widen(*p) + s * a.scale);
 }
 
-template <typename TD>
-__global__ void __launch_bounds__(256) k_zero_rows(TD* p, uint64_t rows, uint64_t d, uint64_t ld) {
-  for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (uint64_t c = threadIdx.x; c < d; c += blockDim.x) p[r * ld + c] = rw_round<TD>(0.0f);
+__global__ void __launch_bounds__(kCountThreads) k_zero_rows(ZeroRows z) {
+  zero_units(z, (uint64_t)blockIdx.x * kCountThreads + threadIdx.x, (uint64_t)gridDim.x * kCountThreads);
 }
 
 // =================================================================================
@@ -749,6 +775,26 @@ GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
 
 }  // namespace
 
+namespace {
+
+ZeroRows zero_rows(const EmbedGradLaunch& a) {
+  const uint64_t elem = rw_type_bytes(a.dtable_type), pitch = a.ld_dtable * elem;
+  ZeroRows z = {(char*)a.dtable, a.vocab, 0, pitch, (uint32_t)elem};
+  uint64_t bytes = a.d * elem;
+  if (a.vocab == 1 || a.ld_dtable == a.d) {  // one run
+    bytes *= a.vocab;
+    z.rows = 1;
+  }
+  if (bytes % 16 == 0 && (uintptr_t)a.dtable % 16 == 0 && (z.rows == 1 || pitch % 16 == 0)) z.unit = 16;
+  z.row_units = bytes / z.unit;
+  return z;
+}
+uint32_t zero_ctas(const ZeroRows& z) {
+  return grid_of((z.rows * z.row_units + 4 * kCountThreads - 1) / (4 * kCountThreads), 8);
+}
+
+}  // namespace
+
 uint64_t embed_grad_workspace(uint64_t n, uint64_t d, uint64_t vocab) {
   return n == 0 || d == 0 || vocab == 0 ? 0 : grad_plan(n, d, vocab).bytes;
 }
@@ -759,11 +805,8 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   if (a.n == 0) {
     if (a.accumulate) return cudaSuccess;
     *nl += 1;
-    return rw_with_type(a.dtable_type, [&](auto td) {
-      using TD = decltype(td);
-      return rw_launch(k_zero_rows<TD>, dim3(grid_of(a.vocab, 8)), dim3(256), 0, s, false,
-                       (TD*)a.dtable, a.vocab, a.d, a.ld_dtable);
-    });
+    const ZeroRows z = zero_rows(a);
+    return rw_launch(k_zero_rows, dim3(zero_ctas(z)), dim3(kCountThreads), 0, s, false, z);
   }
   const GradPlan g = grad_plan(a.n, a.d, a.vocab);
   char* ws = (char*)workspace;
@@ -789,13 +832,18 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   unsigned long long* buf[2] = {(unsigned long long*)(ws + g.pairs0),
                                 (unsigned long long*)(ws + g.pairs1)};
   const bool count = a.n <= kCountSort;
+  // Few ids, many rows: the whole table is zeroed beside the sort and the rows that ids name
+  // are written again, instead of looking for each row among the ids (512 ids into 32000 x
+  // 768: 30 -> 21 us).
+  const bool zero_first = count && !a.accumulate && a.n <= a.vocab / 8;
   if (count) {
     *nl += 1;
     e = rw_with_index(a.id_type, [&](auto id) {
       using ID = decltype(id);
       const uint32_t blocks = (uint32_t)((a.n * kCountShare + kCountThreads - 1) / kCountThreads);
-      return rw_launch(k_token_rank<ID>, dim3(blocks), dim3(kCountThreads), 0, s, false,
-                       (const ID*)a.ids, (uint32_t)a.n, (uint32_t)a.vocab, buf[0]);
+      const ZeroRows z = zero_rows(a);
+      return rw_launch(k_token_rank<ID>, dim3(blocks + (zero_first ? zero_ctas(z) : 0)), dim3(kCountThreads),
+                       0, s, false, (const ID*)a.ids, (uint32_t)a.n, (uint32_t)a.vocab, buf[0], blocks, z);
     });
   }
   SortPass p = {};
@@ -833,7 +881,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
       const bool wide = rw_packs(a.grad, a.n, a.d, a.ld_grad, sizeof(TG), kV) &&
                         rw_packs(a.dtable, a.vocab, a.d, a.ld_dtable, sizeof(TD), kV);
       cp = chunk_plan(a.n, a.d, wide ? kV : 1);
-      const uint64_t zero = a.accumulate ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
+      const uint64_t zero = a.accumulate || zero_first ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
       const dim3 grid((uint32_t)(cp.sum_ctas + zero));
       return wide ? rw_launch(k_embed_chunks<TG, TD, kV>, grid, dim3(kSumThreads), 0, s, true, a, cp,
                               pairs, partial)

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
-constexpr uint32_t kGroups = 128;  // groups of threads whose maxima bound the top places
+constexpr uint32_t kGroups = 64;   // groups of threads whose maxima bound the top places
 constexpr uint32_t kCand = 1024;   // candidates for the top places that a CTA keeps
 constexpr uint32_t kRare = 2 * kMaxTop;  // threads that reach the bound, if few margins equal it
 constexpr uint32_t kMaxParts = 64;
@@ -326,35 +326,44 @@ struct TopSpace {
   uint32_t count, bound;
 };
 
-// The top_k places among the span's margins, in order, given every thread's largest margin;
+// The first two steps of top_places, each followed by a barrier of the caller's: every
+// thread's largest margin, and the groups' largest. The threads of a group are far apart, so
+// neighbours in a row fall into different groups.
+constexpr uint32_t kGroupSize = kRowThreads / kGroups;
+__device__ __forceinline__ void top_threads(float own, TopSpace& s) {
+  s.order[threadIdx.x] = order_of(own);
+  if (threadIdx.x == 0) s.count = 0;
+}
+__device__ __forceinline__ void top_groups(TopSpace& s) {
+  const uint32_t t = threadIdx.x;
+  if (t < kGroups) {
+    uint32_t g = s.order[t];
+#pragma unroll
+    for (uint32_t q = 1; q < kGroupSize; q++) g = max(g, s.order[t + q * kGroups]);
+    s.group[t] = g;
+  }
+}
+
+// The top_k places among the span's margins, in order, after top_threads and top_groups;
 // emit(place, key) is called once a place. All threads of the CTA call it.
 template <typename T, typename Emit>
 __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32_t top_k, TopSpace& s, Emit emit) {
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   constexpr int kV = Span<T>::kV;
   const uint32_t mine = order_of(own);
-  __syncthreads();
-  s.order[t] = mine;
-  if (t == 0) s.count = 0;
-  __syncthreads();
-  // A bound that top_k margins at least reach: the top_k-th largest of the groups' maxima.
-  // The threads of a group are far apart, so neighbours in a row fall into different groups.
-  if (t < kGroups) {
-    uint32_t g = s.order[t];
-#pragma unroll
-    for (uint32_t q = t + kGroups; q < kRowThreads; q += kGroups) g = max(g, s.order[q]);
-    s.group[t] = g;
-  }
-  __syncthreads();
-  if (t < kGroups) {
-    const uint32_t g = s.group[t];
+  // A bound that top_k margins at least reach: the top_k-th largest of the groups' maxima,
+  // found by counting; the kGroupSize threads of a group share the comparisons.
+  {
+    const uint32_t at = t / kGroupSize, g = s.group[at];
     uint32_t above = 0;
-#pragma unroll 8
-    for (uint32_t q = 0; q < kGroups; q++) {
-      const uint32_t o = s.group[q];
-      above += o > g || (o == g && q < t);
+#pragma unroll
+    for (uint32_t u = 0; u < kGroups / kGroupSize; u++) {
+      const uint32_t q = t % kGroupSize + u * kGroupSize, o = s.group[q];
+      above += o > g || (o == g && q < at);
     }
-    if (above == top_k - 1) s.bound = g;
+#pragma unroll
+    for (uint32_t o = kGroupSize / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (above == top_k - 1) s.bound = g;  // one group's threads
   }
   __syncthreads();
   const uint32_t bound = s.bound;
@@ -399,6 +408,7 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
     for (uint32_t q = t; q < count; q += kRowThreads) {
       const Key k = s.cand[q];
       uint32_t place = 0;
+#pragma unroll 8
       for (uint32_t w = 0; w < count; w++) place += s.cand[w] > k;
       if (place < top_k) emit(place, k);
     }
@@ -577,7 +587,9 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
     r = join(r, one, c);
   }
   const float own = r.m;
+  if (a.top_k) top_threads(own, s_top);
   const float all = cta_max(own, s_max);
+  if (a.top_k) top_groups(s_top);
   if (all != -kInf) {
     if ((all <= kLowest) || !(a.scale >= kScaleLow && a.scale <= kScaleHigh)) {
       r.s = r.t = 0.0f;
@@ -611,50 +623,58 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
 
 // Joins a split row: the parts' sums, and the top places of their sorted lists (a list whose
 // head is below the top_k-th largest head has none).
+constexpr int kJoinThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(256) k_logprobs_join(LogprobsLaunch a, SplitRow sr) {
+__global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a, SplitRow sr) {
   __shared__ Key s_head[kMaxParts];
   __shared__ Key s_cand[kMaxTop * kMaxTop + kMaxTop];
   __shared__ uint32_t s_count;
   __shared__ Key s_bound;
+  constexpr int kHeld = kMaxParts * kMaxTop / kJoinThreads;  // keys a thread holds
   const uint32_t t = threadIdx.x, lane = t & 31;
   const uint64_t i = blockIdx.x;
   const float c = a.scale * kLog2e;
   rw_dependent_start();
+  // everything that is read is on its way before anything is waited for
   const Sums* sums = sr.sums + i * sr.parts;
-  Sums r;
+  Sums r, r2;
   if (lane < sr.parts) r = sums[lane];
-  if (lane + 32 < sr.parts) r = join(r, sums[lane + 32], c);
+  if (lane + 32 < sr.parts) r2 = sums[lane + 32];
+  const uint32_t cells = sr.parts * a.top_k;
+  const Key* keys = sr.keys + i * cells;
+  Key held[kHeld];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
-  const RowEnd end = row_end(r);
-  if (t == 0) write_row<T>(a, i, r, end);
-  if (a.top_k == 0) return;
-  const Key* keys = sr.keys + i * sr.parts * a.top_k;
-  if (t < sr.parts) s_head[t] = keys[(uint64_t)t * a.top_k];
+  for (int u = 0; u < kHeld; u++) held[u] = t + u * kJoinThreads < cells ? keys[t + u * kJoinThreads] : 0;
+  if (t < sr.parts && a.top_k) s_head[t] = keys[(uint64_t)t * a.top_k];
   if (t == 0) {
     s_count = 0;
     s_bound = 1;  // fewer lists than places: every key counts
   }
+  r = join(r, r2, c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
+  const RowEnd end = row_end(r);
+  if (t == kJoinThreads - 1) write_row<T>(a, i, r, end);  // the warp with the least to do below
+  if (a.top_k == 0) return;
   __syncthreads();
   if (sr.parts >= a.top_k && t < sr.parts) {
     uint32_t above = 0;
+#pragma unroll 8
     for (uint32_t q = 0; q < sr.parts; q++) above += s_head[q] > s_head[t];
     if (above == a.top_k - 1) s_bound = s_head[t];
   }
   __syncthreads();
+  // at most top_k lists have a head at the bound or above, so at most top_k^2 keys do
   const Key bound = s_bound;
-  // at most top_k lists have a head at the bound or above
-  for (uint32_t q = t; q < sr.parts * a.top_k; q += 256) {
-    if (s_head[q / a.top_k] < bound) continue;
-    const Key k = keys[q];
-    if (k >= bound) s_cand[atomicAdd(&s_count, 1u)] = k;
-  }
+#pragma unroll
+  for (int u = 0; u < kHeld; u++)
+    if (held[u] >= bound) s_cand[atomicAdd(&s_count, 1u)] = held[u];
   __syncthreads();
   const uint32_t count = s_count;
-  for (uint32_t q = t; q < count; q += 256) {
+  for (uint32_t q = t; q < count; q += kJoinThreads) {
     const Key k = s_cand[q];
     uint32_t place = 0;
+#pragma unroll 8
     for (uint32_t w = 0; w < count; w++) place += s_cand[w] > k;
     if (place < a.top_k) write_top(a, i, place, k, end);
   }
@@ -870,7 +890,7 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
                               : rw_launch(k_logprobs_row<T, false>, grid, block, 0, s, false, a, r);
     if (e != cudaSuccess || r.parts == 1) return e;
     *nl += 1;
-    return rw_launch(k_logprobs_join<T>, dim3((uint32_t)a.n), dim3(256), 0, s, true, a, r);
+    return rw_launch(k_logprobs_join<T>, dim3((uint32_t)a.n), dim3(kJoinThreads), 0, s, true, a, r);
   });
 }
 
