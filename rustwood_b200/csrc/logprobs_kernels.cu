@@ -43,10 +43,11 @@ __device__ __forceinline__ float exp2_fast(float v) {
 }
 
 // An order of the margins as whole numbers above 0 (NaN above +inf, -0 equal to +0), and with
-// the index below it: larger margins first, lower indices first among equal ones.
+// the index below it: larger margins first, lower indices first among equal ones. The
+// addition makes -0 into +0 and every NaN into the one with all bits but the sign set.
 __device__ __forceinline__ uint32_t order_of(float x) {
-  const uint32_t b = __float_as_uint(x + 0.0f);
-  return x != x ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
+  const uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float margin_of(uint32_t order) {
   return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
@@ -99,7 +100,7 @@ __device__ __forceinline__ void write_row(const LogprobsLaunch& a, uint64_t i, c
   if (a.row_max) a.row_max[i] = r.m;
   if (a.log_sum) a.log_sum[i] = e.log_sum;
   if (a.lse) a.lse[i] = a.scale * r.m + e.log_sum;
-  if (a.entropy) a.entropy[i] = r.m == -kInf ? 0.0f : e.log_sum - a.scale * (r.t / r.s);
+  if (a.entropy) a.entropy[i] = r.m == -kInf ? 0.0f : e.log_sum - a.scale * __fdividef(r.t, r.s);
   if (a.logp) {
     const int64_t c = a.target_type == RW_I64 ? ((const int64_t*)a.targets)[i] : ((const int32_t*)a.targets)[i];
     float v = 0.0f;
@@ -194,18 +195,26 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
         continue;
       }
     }
-    Key last = ~0ull;
-    for (uint32_t place = 0; place < a.top_k; place++) {
-      Key best = 0;
+    // place by place; a margin that has its place has order 0 from then on
+    uint32_t order[E];
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const uint32_t j = lane + e * L;
-        const Key k = j < classes ? key_of(order_of(v[e]), j) : 0;
-        if (k < last && k > best) best = k;
+    for (int e = 0; e < E; e++) order[e] = lane + e * L < classes ? order_of(v[e]) : 0;
+    for (uint32_t place = 0; place < a.top_k; place++) {
+      uint32_t top = order[0], at = lane;
+#pragma unroll
+      for (int e = 1; e < E; e++) {
+        if (order[e] > top) {
+          top = order[e];
+          at = lane + e * L;
+        }
       }
+      Key best = key_of(top, at);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-      last = best;
+      at = index_of(best);
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (lane + e * L == at) order[e] = 0;
       if (real && lane == 0) write_top(a, i, place, best, end);
     }
   }
@@ -219,7 +228,9 @@ constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
 constexpr uint32_t kGroups = 64;   // groups of threads whose maxima bound the top places
 constexpr uint32_t kCand = 1024;   // candidates for the top places that a CTA keeps
-constexpr uint32_t kRare = 2 * kMaxTop;  // threads that reach the bound, if few margins equal it
+// Threads that hold a margin above the bound are fewer than top_k groups'. With more that
+// reach it, many margins equal it.
+constexpr uint32_t kLook = kMaxTop * (kRowThreads / kGroups);
 constexpr uint32_t kMaxParts = 64;
 
 // Where a row's sums and top keys are left when it is split: [row][part].
@@ -323,7 +334,8 @@ struct TopSpace {
   Key cand[kCand];
   uint32_t warp[kRowWarps];
   Key warp_key[kRowWarps];
-  uint32_t count, bound;
+  uint32_t look[kLook];
+  uint32_t count, bound, looking;
 };
 
 // The first two steps of top_places, each followed by a barrier of the caller's: every
@@ -332,7 +344,7 @@ struct TopSpace {
 constexpr uint32_t kGroupSize = kRowThreads / kGroups;
 __device__ __forceinline__ void top_threads(float own, TopSpace& s) {
   s.order[threadIdx.x] = order_of(own);
-  if (threadIdx.x == 0) s.count = 0;
+  if (threadIdx.x == 0) s.count = s.looking = 0;
 }
 __device__ __forceinline__ void top_groups(TopSpace& s) {
   const uint32_t t = threadIdx.x;
@@ -367,29 +379,36 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
   }
   __syncthreads();
   const uint32_t bound = s.bound;
-  // Collects the margins whose order is at least `from`: a warp reads again, with all its
-  // lanes, the vectors of each thread that has one.
+  // Collects the margins whose order is at least `from`: the threads that have one are
+  // listed and their vectors read again, spread over all threads. False: too many have one.
   auto collect = [&](uint32_t from) {
+    if (mine >= from) {
+      const uint32_t at = atomicAdd(&s.looking, 1u);
+      if (at < kLook) s.look[at] = t;
+    }
+    __syncthreads();
+    const uint32_t looking = s.looking;
+    if (looking > kLook) return false;
     auto offer = [&](float x, uint32_t j) {
       const uint32_t o = order_of(x);
       if (o < from) return;
       const uint32_t at = atomicAdd(&s.count, 1u);
       if (at < kCand) s.cand[at] = key_of(o, offset + j);
     };
-    for (uint32_t who = __ballot_sync(0xffffffffu, mine >= from); who; who &= who - 1) {
-      const uint32_t first = warp * 32 + __ffs(who) - 1;
-      for (uint32_t v = first + lane * kRowThreads; v < sp.vecs; v += 32 * kRowThreads) {
-        Pack<T, kV> p;
-        p.load(sp.vec(v));
-        if (order_of(pack_max(p)) < from) continue;
+    const uint32_t each = (sp.vecs + kRowThreads - 1) / kRowThreads;
+    for (uint32_t q = t; q < looking * each; q += kRowThreads) {
+      const uint32_t who = q / each, v = s.look[who] + (q - who * each) * kRowThreads;
+      if (v >= sp.vecs) continue;
+      Pack<T, kV> p;
+      p.load(sp.vec(v));
+      if (order_of(pack_max(p)) < from) continue;
 #pragma unroll
-        for (int k = 0; k < kV; k++) offer(p.get(k), sp.head + v * kV + k);
-      }
+      for (int k = 0; k < kV; k++) offer(p.get(k), sp.head + v * kV + k);
     }
     if (t < sp.ragged()) offer(rw_widen(sp.x[sp.ragged_at(t)]), sp.ragged_at(t));
+    return true;
   };
-  const bool rare = __syncthreads_count(mine >= bound) <= (int)kRare;
-  if (rare) collect(bound);
+  const bool rare = collect(bound);
   __syncthreads();
   uint32_t count = s.count;
   uint32_t ties = 0;  // places that go to margins equal to the bound, in index order
@@ -397,7 +416,7 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
     // Many margins equal to the bound (a mask, a constant row): only those above it are
     // candidates, and the first of the equal ones follow.
     __syncthreads();
-    if (t == 0) s.count = 0;
+    if (t == 0) s.count = s.looking = 0;
     __syncthreads();
     if (bound != 0xffffffffu) collect(bound + 1);
     __syncthreads();
@@ -502,6 +521,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
   const uint32_t part = blockIdx.x % sr.parts;
   const uint64_t lo = part * sr.part, hi = min(lo + sr.part, a.classes);
   const Span<T> sp((const T*)a.x + i * a.ld_x + lo, (uint32_t)(hi - lo));
+  rw_let_successor_start();  // k_logprobs_join of a split row waits for this kernel
   const float c = a.scale * kLog2e;
 
   float m = -kInf, mc = 0.0f;
@@ -621,17 +641,19 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
   }
 }
 
-// Joins a split row: the parts' sums, and the top places of their sorted lists (a list whose
-// head is below the top_k-th largest head has none).
+// Joins a split row: the parts' sums, and the top places of their sorted lists. The p-th of a
+// list whose head has r heads above it has p + r keys above it, and no key below the
+// top_k-th largest head has a place, so few keys need comparing.
 constexpr int kJoinThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a, SplitRow sr) {
   __shared__ Key s_head[kMaxParts];
-  __shared__ Key s_cand[kMaxTop * kMaxTop + kMaxTop];
+  __shared__ uint32_t s_above[kMaxParts];
+  __shared__ Key s_cand[kMaxTop * (kMaxTop + 1) / 2];
   __shared__ uint32_t s_count;
   __shared__ Key s_bound;
-  constexpr int kHeld = kMaxParts * kMaxTop / kJoinThreads;  // keys a thread holds
-  const uint32_t t = threadIdx.x, lane = t & 31;
+  constexpr int kHeld = kMaxParts / (kJoinThreads / 32);  // a list a warp, a key a lane
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint64_t i = blockIdx.x;
   const float c = a.scale * kLog2e;
   rw_dependent_start();
@@ -640,35 +662,40 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
   Sums r, r2;
   if (lane < sr.parts) r = sums[lane];
   if (lane + 32 < sr.parts) r2 = sums[lane + 32];
-  const uint32_t cells = sr.parts * a.top_k;
-  const Key* keys = sr.keys + i * cells;
+  const Key* keys = sr.keys + i * sr.parts * a.top_k;
   Key held[kHeld];
 #pragma unroll
-  for (int u = 0; u < kHeld; u++) held[u] = t + u * kJoinThreads < cells ? keys[t + u * kJoinThreads] : 0;
+  for (int u = 0; u < kHeld; u++) {
+    const uint32_t list = warp + u * (kJoinThreads / 32);
+    held[u] = list < sr.parts && lane < a.top_k ? keys[list * a.top_k + lane] : 0;
+  }
   if (t < sr.parts && a.top_k) s_head[t] = keys[(uint64_t)t * a.top_k];
   if (t == 0) {
     s_count = 0;
-    s_bound = 1;  // fewer lists than places: every key counts
+    s_bound = 1;  // with fewer lists than places only the ends of short lists, 0, are below
   }
   r = join(r, r2, c);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
   const RowEnd end = row_end(r);
-  if (t == kJoinThreads - 1) write_row<T>(a, i, r, end);  // the warp with the least to do below
-  if (a.top_k == 0) return;
+  if (a.top_k == 0) {
+    if (t == 0) write_row<T>(a, i, r, end);
+    return;
+  }
   __syncthreads();
-  if (sr.parts >= a.top_k && t < sr.parts) {
+  if (t < sr.parts) {
     uint32_t above = 0;
 #pragma unroll 8
     for (uint32_t q = 0; q < sr.parts; q++) above += s_head[q] > s_head[t];
+    s_above[t] = above;
     if (above == a.top_k - 1) s_bound = s_head[t];
   }
   __syncthreads();
-  // at most top_k lists have a head at the bound or above, so at most top_k^2 keys do
-  const Key bound = s_bound;
 #pragma unroll
-  for (int u = 0; u < kHeld; u++)
-    if (held[u] >= bound) s_cand[atomicAdd(&s_count, 1u)] = held[u];
+  for (int u = 0; u < kHeld; u++) {
+    if (held[u] < s_bound) continue;
+    if (lane + s_above[warp + u * (kJoinThreads / 32)] < a.top_k) s_cand[atomicAdd(&s_count, 1u)] = held[u];
+  }
   __syncthreads();
   const uint32_t count = s_count;
   for (uint32_t q = t; q < count; q += kJoinThreads) {
@@ -678,6 +705,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
     for (uint32_t w = 0; w < count; w++) place += s_cand[w] > k;
     if (place < a.top_k) write_top(a, i, place, k, end);
   }
+  if (t == kJoinThreads - 1) write_row<T>(a, i, r, end);  // the warp with the least to do above
 }
 
 // =================================================================================
@@ -701,10 +729,9 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobsGradLaunch& a, uint64_
   float g = 0.0f;
   if (a.targets) {
     const int64_t t = a.target_type == RW_I64 ? ((const int64_t*)a.targets)[i] : ((const int32_t*)a.targets)[i];
-    if (t >= 0 && (uint64_t)t < a.classes) {
-      r.target = (int32_t)t;
-      g = a.grad_logp[i];
-    }
+    g = a.grad_logp[i];  // on its way whatever the target is
+    if (t >= 0 && (uint64_t)t < a.classes) r.target = (int32_t)t;
+    else g = 0.0f;
   }
   const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f;
   if (g == 0.0f && e == 0.0f) return r;
@@ -713,9 +740,15 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobsGradLaunch& a, uint64_
     r.kind = 2;
     return r;
   }
-  const double k = (double)m * (double)(a.scale * kLog2e) + (double)a.log_sum[i] * 1.4426950408889634;
-  r.k = (float)k;
-  const float rest = (float)(k - (double)r.k), f = exp2_fast(-rest) * a.scale;
+  // k = m c + log_sum log2(e) in two f32: products and sum with their roundings
+  constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
+  const float c = a.scale * kLog2e, s = a.log_sum[i];
+  const float mc = m * c, sl = s * kLog2e;
+  const float k = mc + sl, back = k - mc;
+  const float rest = ((mc - (k - back)) + (sl - back)) +
+                     (__fmaf_rn(m, c, -mc) + __fmaf_rn(s, kLog2e, -sl) + s * kLog2eRest);
+  const float f = exp2_fast(-rest) * a.scale;
+  r.k = k;
   const float h = a.grad_entropy ? a.entropy[i] : 0.0f;
   constexpr float kLn2 = 0.6931471805599453f;
   r.a = f * (g + e * (h - rest * kLn2));
@@ -796,41 +829,60 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaun
 
 // Few classes: a CTA takes `rows` whole rows, their constants in shared memory. VEC: the
 // matrices are contiguous and aligned, so the rows are one run of 16-byte vectors whose
-// elements may lie in different rows.
+// elements may lie in different rows. magic = ceil(2^32 / classes): an element's row is the
+// high half of its index times magic, exactly, as index * classes < 2^32.
 constexpr uint32_t kGradRows = 1024;
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGradLaunch a, uint32_t rows) {
-  __shared__ RowGrad s_row[kGradRows];
+__global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGradLaunch a, uint32_t rows, uint32_t magic) {
+  __shared__ float4 s_row[kGradRows];     // k, a, b, hit
+  __shared__ int32_t s_target[kGradRows];  // -1: none, -2: a row of zeros
   constexpr int kV = VEC ? 16 / (int)sizeof(T) : 1;
   const uint64_t first = (uint64_t)blockIdx.x * rows;
   const uint32_t count = (uint32_t)min((uint64_t)rows, a.n - first), classes = (uint32_t)a.classes;
-  for (uint32_t k = threadIdx.x; k < count; k += kGradThreads) s_row[k] = row_grad(a, first + k);
-  __syncthreads();
   const float c = a.scale * kLog2e;
   const uint32_t total = count * classes;
   const T* x = (const T*)a.x + first * a.ld_x;
   T* dx = (T*)a.dx + first * a.ld_dx;
+  bool formula = false;
+  for (uint32_t k = threadIdx.x; k < count; k += kGradThreads) {
+    const RowGrad r = row_grad(a, first + k);
+    s_row[k] = make_float4(r.k, r.a, r.b, r.hit);
+    s_target[k] = r.kind ? r.target : -2;
+    formula |= r.kind == 2;
+  }
+  formula = __syncthreads_or(formula);
+  auto element = [&](uint32_t at, uint32_t row, float in) {
+    const uint32_t j = at - row * classes;
+    const float4 r = s_row[row];
+    const int32_t target = s_target[row];
+    const bool hit = (int32_t)j == target;
+    float v;
+    if (formula) {  // every row of the CTA, by the row's own rule
+      v = target == -2 ? 0.0f : grad_element(a, first + row, row_grad(a, first + row), c, in, j);
+    } else {
+      const float d = __fmaf_rn(max_nan(in, kLowest), c, -r.x);
+      v = -exp2_fast(d) * __fmaf_rn(r.z, d, r.y);
+      v = hit ? v + r.w : v;
+      v = target == -2 ? 0.0f : v;
+    }
+    return v;
+  };
+  auto row_of = [&](uint32_t at) { return classes == 1 ? at : __umulhi(at, magic); };
   for (uint32_t j0 = threadIdx.x * kV; j0 < total; j0 += kGradThreads * kV) {
-    uint32_t row = j0 / classes, j = j0 - row * classes;
-    RowGrad r = s_row[row];
-    Pack<T, kV> p;
-    const bool all = VEC && j0 + kV <= total;
-    if (all) p.load(x + j0);
+    if (VEC && j0 + kV <= total) {
+      Pack<T, kV> p;
+      p.load(x + j0);
 #pragma unroll
-    for (int k = 0; k < kV; k++) {
-      if (!all && j0 + k >= total) break;
-      const size_t from = VEC ? j0 + k : row * a.ld_x + j, to = VEC ? j0 + k : row * a.ld_dx + j;
-      const float in = all ? p.get(k) : rw_widen(x[from]);
-      const float v = r.kind ? grad_element(a, first + row, r, c, in, j) : 0.0f;
-      if (all) p.set(k, v);
-      else dx[to] = rw_round<T>(v);
-      if (kV > 1 && ++j == classes && j0 + k + 1 < total) {
-        j = 0;
-        r = s_row[++row];
+      for (int k = 0; k < kV; k++) p.set(k, element(j0 + k, row_of(j0 + k), p.get(k)));
+      p.store(dx + j0);
+    } else {
+      for (uint32_t at = j0; at < min(total, j0 + kV); at++) {
+        const uint32_t row = row_of(at), j = at - row * classes;
+        const size_t from = VEC ? at : row * a.ld_x + j, to = VEC ? at : row * a.ld_dx + j;
+        dx[to] = rw_round<T>(element(at, row, rw_widen(x[from])));
       }
     }
-    if (all) p.store(dx + j0);
   }
 }
 
@@ -913,8 +965,10 @@ cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, in
       rows = std::min<uint64_t>(std::max<uint64_t>(rows, 1) + kV - 1, kGradRows) / kV * kV;
       const uint64_t ctas = (a.n + rows - 1) / rows;
       if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
-      return vec ? rw_launch(k_logprobs_grad_few<T, true>, dim3((uint32_t)ctas), block, 0, s, false, a, (uint32_t)rows)
-                 : rw_launch(k_logprobs_grad_few<T, false>, dim3((uint32_t)ctas), block, 0, s, false, a, (uint32_t)rows);
+      const uint32_t magic = (uint32_t)(((1ull << 32) + a.classes - 1) / a.classes);
+      const dim3 grid((uint32_t)ctas);
+      return vec ? rw_launch(k_logprobs_grad_few<T, true>, grid, block, 0, s, false, a, (uint32_t)rows, magic)
+                 : rw_launch(k_logprobs_grad_few<T, false>, grid, block, 0, s, false, a, (uint32_t)rows, magic);
     }
     const bool vec = x % 16 == dx % 16 && (one || (a.ld_x * sizeof(T)) % 16 == (a.ld_dx * sizeof(T)) % 16);
     const uint64_t per = kGradThreads * kGradDepth * kV, chunks = (a.classes + per - 1) / per;

@@ -126,8 +126,11 @@ __device__ __forceinline__ T rw_load_here(const T* p) {
 
 // Programmatic dependent launch: a kernel launched as `dependent` (rw_launch) lets its
 // successor start, then waits until its predecessors' writes are visible.
-__device__ __forceinline__ void rw_dependent_start() {
+__device__ __forceinline__ void rw_let_successor_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void rw_dependent_start() {
+  rw_let_successor_start();
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
