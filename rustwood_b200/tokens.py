@@ -88,7 +88,7 @@ def _output(ctx: Context, out: Optional[torch.Tensor], shape, dtype: torch.dtype
             device: torch.device) -> tuple[torch.Tensor, int]:
     """The output tensor and the distance of its rows."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device), shape[-1]
+        return torch.empty(*shape, dtype=dtype, device=device), shape[-1]
     _on_gpu(ctx, "out", out)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"out is {tuple(out.shape)} {out.dtype}: {tuple(shape)} {dtype} is needed")
@@ -192,9 +192,9 @@ def logprobs(ctx: Context, x: torch.Tensor, targets: Optional[torch.Tensor] = No
     shape, device = x.shape[:-1], rows.device
     t, target_kind = (None, N.RW_I64) if targets is None else _index(ctx, "targets", targets, n)
     need = _bytes_needed("rw_logprobs_workspace", n, classes, kind, top_k)
-    row = torch.empty((5, *shape), dtype=torch.float32, device=device)
-    top_logp = torch.empty((*shape, top_k), dtype=torch.float32, device=device)
-    top_index = torch.empty((*shape, top_k), dtype=torch.int64, device=device)
+    row = torch.empty(5, *shape, dtype=torch.float32, device=device)
+    top_logp = torch.empty(*shape, top_k, dtype=torch.float32, device=device)
+    top_index = torch.empty(*shape, top_k, dtype=torch.int64, device=device)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     at, step = row.data_ptr(), 4 * n
     ctx.check(N.lib.rw_logprobs_device(
