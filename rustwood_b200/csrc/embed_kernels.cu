@@ -22,10 +22,10 @@ constexpr int kSms = 148;
 // =================================================================================
 // lookup
 
-// A CTA takes `slots` rows at a time, `tx` threads a row, V columns a thread and kEmbedDepth
-// vectors in flight: one pass, each id read once per row of threads.
+// `tx` threads a row, V columns a thread and access; a thread takes R rows and C vectors of
+// each at a time, all in flight, so that short rows have as much in flight as long ones. Every
+// CTA takes slots * R rows and is done.
 constexpr int kEmbedThreads = 256;
-constexpr int kEmbedDepth = 4;
 
 struct EmbedPlan {
   uint32_t tx, slots;
@@ -33,31 +33,46 @@ struct EmbedPlan {
   uint32_t split;  // CTAs that share a row's columns
 };
 
-template <typename TI, typename TO, typename ID, int V>
+template <typename TI, typename TO, int V, int R, int C>
 __global__ void __launch_bounds__(kEmbedThreads) k_embed(EmbedLaunch a, EmbedPlan ep) {
   const uint32_t slot = threadIdx.x / ep.tx, lane = threadIdx.x % ep.tx;
   if (slot >= ep.slots) return;
-  const TI* table = (const TI*)a.table;
-  const ID* ids = (const ID*)a.ids;
   const uint64_t step = (uint64_t)ep.tx * ep.split;
   const uint64_t first = (uint64_t)(blockIdx.x % ep.split) * ep.tx + lane;
-  for (uint64_t i = (uint64_t)(blockIdx.x / ep.split) * ep.slots + slot; i < a.n;
-       i += (uint64_t)(gridDim.x / ep.split) * ep.slots) {
-    const int64_t id = (int64_t)ids[i];
-    const bool in = id >= 0 && (uint64_t)id < a.vocab;
-    const TI* row = table + (in ? (uint64_t)id : 0) * a.ld_table;
-    TO* out = (TO*)a.out + i * a.ld_out;
-    for (uint64_t c = first; c < ep.dv; c += step * kEmbedDepth) {
-      Pack<TI, V> v[kEmbedDepth];
+  const uint64_t i0 = (uint64_t)(blockIdx.x / ep.split) * ep.slots * R + slot;
+  int64_t id[R];
 #pragma unroll
-      for (int u = 0; u < kEmbedDepth; u++)
-        if (in && c + u * step < ep.dv) v[u].load(row + (c + u * step) * V);
+  for (int r = 0; r < R; r++) {
+    const uint64_t i = i0 + (uint64_t)r * ep.slots;
+    id[r] = -1;
+    if (i < a.n) id[r] = a.id_type == RW_I64 ? ((const int64_t*)a.ids)[i] : ((const int32_t*)a.ids)[i];
+    if (id[r] >= 0 && (uint64_t)id[r] >= a.vocab) id[r] = -1;
+  }
+  for (uint64_t c = first; c < ep.dv; c += step * C) {
+    Pack<TI, V> v[R][C];
 #pragma unroll
-      for (int u = 0; u < kEmbedDepth; u++) {
+    for (int r = 0; r < R; r++) {
+      const TI* row = (const TI*)a.table + (uint64_t)max(id[r], (int64_t)0) * a.ld_table;
+#pragma unroll
+      for (int u = 0; u < C; u++)
+        if (id[r] >= 0 && c + u * step < ep.dv) v[r][u].load(row + (c + u * step) * V);
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const uint64_t i = i0 + (uint64_t)r * ep.slots;
+      if (i >= a.n) break;
+      TO* out = (TO*)a.out + i * a.ld_out;
+#pragma unroll
+      for (int u = 0; u < C; u++) {
         if (c + u * step >= ep.dv) break;
         Pack<TO, V> o;
+        if (id[r] >= 0) {
 #pragma unroll
-        for (int k = 0; k < V; k++) o.set(k, in ? a.scale * v[u].get(k) : 0.0f);
+          for (int k = 0; k < V; k++) o.set(k, a.scale * v[r][u].get(k));
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; k++) o.set(k, 0.0f);
+        }
         o.store_streaming(out + (c + u * step) * V);
       }
     }
@@ -675,43 +690,52 @@ __device__ __forceinline__ Words philox(uint64_t group, uint64_t sequence, const
   return {{c0, c1, c2, c3}};
 }
 
-__device__ __forceinline__ bool dropout_keep(const Words& w, int k, uint32_t limit) {
-  return (k & 1 ? w.w[k / 2] >> 16 : w.w[k / 2] & 0xffff) >= limit;
+// high_limit = limit << 16: the other half of the word does not change the comparison.
+__device__ __forceinline__ bool dropout_keep(const Words& w, int k, uint32_t high_limit) {
+  return (k & 1 ? w.w[k / 2] : w.w[k / 2] << 16) >= high_limit;
 }
 
-// One thread takes the 8 elements of a counter, two counters at a time so that two loads are
-// in flight while it computes. VEC: the matrices are contiguous and 16-byte aligned, so a
+constexpr int kDropoutCtas = 5;
+template <typename T>
+constexpr int kDropoutDepth = 8 / (int)sizeof(T);  // 64 bytes
+
+// One thread takes the 8 elements of a counter, kDropoutDepth counters whose loads are all in
+// flight before it computes, and is done: many short CTAs overlap better than a resident grid
+// that walks the matrix with as many loads in flight (268M bf16: 185 us, 5.8 TB/s, against
+// 209-221 us). VEC: the matrices are contiguous and 16-byte aligned, so a
 // group is one or two 16-byte accesses; the last, partial one goes element by element.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_dropout(DropoutLaunch a, PhiloxKeys keys) {
+__global__ void __launch_bounds__(256, kDropoutCtas) k_dropout(DropoutLaunch a, PhiloxKeys keys) {
   const uint64_t total = a.rows * a.cols;
+  const uint32_t limit = a.limit << 16;  // p = 1 does not come here
   const T* x = (const T*)a.x;
   T* y = (T*)a.y;
   const uint64_t t = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const uint64_t threads = (uint64_t)gridDim.x * blockDim.x;
+  constexpr int kDepth = kDropoutDepth<T>;
   if (VEC) {
     const uint64_t whole = total / 8;
-    for (uint64_t g = t; g < whole; g += 2 * threads) {
-      const bool two = g + threads < whole;
-      Pack<T, 8> v[2];
-      v[0].load(x + g * 8);
-      if (two) v[1].load(x + (g + threads) * 8);
+    const uint64_t first = (uint64_t)blockIdx.x * (256 * kDepth) + threadIdx.x;
+    Pack<T, 8> v[kDepth];
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-        if (b && !two) break;
-        const Words w = philox(g + b * threads, a.sequence, keys);
+    for (int b = 0; b < kDepth; b++)
+      if (first + b * 256 < whole) v[b].load(x + (first + b * 256) * 8);
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-          v[b].set(k, dropout_keep(w, k, a.limit) ? v[b].get(k) * a.scale : 0.0f);
-        v[b].store(y + (g + b * threads) * 8);
-      }
+    for (int b = 0; b < kDepth; b++) {
+      const uint64_t g = first + b * 256;
+      if (g >= whole) break;
+      const Words w = philox(g, a.sequence, keys);
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        v[b].set(k, dropout_keep(w, k, limit) ? v[b].get(k) * a.scale : 0.0f);
+      v[b].store_streaming(y + g * 8);
     }
     if (t == 0 && whole * 8 < total) {
       const Words w = philox(whole, a.sequence, keys);
 #pragma unroll
       for (int k = 0; k < 7; k++) {
         const uint64_t e = whole * 8 + k;
-        if (e < total) y[e] = rw_round<T>(dropout_keep(w, k, a.limit) ? rw_widen(x[e]) * a.scale : 0.0f);
+        if (e < total) y[e] = rw_round<T>(dropout_keep(w, k, limit) ? rw_widen(x[e]) * a.scale : 0.0f);
       }
     }
     return;
@@ -723,7 +747,7 @@ __global__ void __launch_bounds__(256) k_dropout(DropoutLaunch a, PhiloxKeys key
     for (int k = 0; k < 8; k++) {
       if (g * 8 + k >= total) break;
       y[r * a.ld_y + c] =
-          rw_round<T>(dropout_keep(w, k, a.limit) ? rw_widen(x[r * a.ld_x + c]) * a.scale : 0.0f);
+          rw_round<T>(dropout_keep(w, k, limit) ? rw_widen(x[r * a.ld_x + c]) * a.scale : 0.0f);
       if (++c == a.cols) {
         c = 0;
         r++;
@@ -738,34 +762,45 @@ uint32_t grid_of(uint64_t blocks, uint32_t per_sm) {
 
 }  // namespace
 
+namespace {
+
+template <typename TI, typename TO, int V>
+cudaError_t embed_launch(const EmbedLaunch& a, cudaStream_t s) {
+  EmbedPlan ep;
+  ep.dv = a.d / V;
+  // few rows: a vector a thread, a row's columns over several CTAs; many: four a thread, of one
+  // row where a row has four warps' worth, else of two or four rows
+  const bool many = a.n >= 8 * kSms;
+  const uint64_t warps = (ep.dv + 31) / 32;
+  const int c = !many ? 1 : warps >= 4 ? 4 : warps >= 2 ? 2 : 1, r = many ? 4 / c : 1;
+  uint64_t tx = ep.dv;
+  if (c > 1) tx = ((ep.dv + c - 1) / c + 31) / 32 * 32;
+  ep.tx = (uint32_t)std::min<uint64_t>(tx, kEmbedThreads);
+  ep.slots = kEmbedThreads / ep.tx;
+  const uint64_t groups = (a.n + ep.slots * r - 1) / (ep.slots * r);
+  const uint64_t most = (ep.dv + ep.tx - 1) / ep.tx;
+  ep.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 2 * kSms / groups));
+  if (groups * ep.split > 0x7fffffffull) return cudaErrorInvalidValue;
+  const dim3 grid((uint32_t)(groups * ep.split)), block(kEmbedThreads);
+  if (c == 4) return rw_launch(k_embed<TI, TO, V, 1, 4>, grid, block, 0, s, false, a, ep);
+  if (c == 2) return rw_launch(k_embed<TI, TO, V, 2, 2>, grid, block, 0, s, false, a, ep);
+  return many ? rw_launch(k_embed<TI, TO, V, 4, 1>, grid, block, 0, s, false, a, ep)
+              : rw_launch(k_embed<TI, TO, V, 1, 1>, grid, block, 0, s, false, a, ep);
+}
+
+}  // namespace
+
 cudaError_t launch_embed(const EmbedLaunch& a, cudaStream_t s, int* nl) {
   if (a.n == 0 || a.d == 0) return cudaSuccess;
   *nl += 1;
   return rw_with_type(a.table_type, [&](auto ti) {
     return rw_with_type(a.out_type, [&](auto to) {
-      return rw_with_index(a.id_type, [&](auto id) {
-        using TI = decltype(ti);
-        using TO = decltype(to);
-        using ID = decltype(id);
-        constexpr int kV = 16 / sizeof(TI);
-        const bool wide = rw_packs(a.table, a.vocab, a.d, a.ld_table, sizeof(TI), kV) &&
-                          rw_packs(a.out, a.n, a.d, a.ld_out, sizeof(TO), kV);
-        EmbedPlan ep;
-        ep.dv = wide ? a.d / kV : a.d;
-        // many rows: kEmbedDepth vectors a thread where a row has a warp's worth of them
-        uint64_t tx = std::min<uint64_t>(ep.dv, kEmbedThreads);
-        if (a.n >= 8 * kSms && ep.dv >= 32 * kEmbedDepth)
-          tx = std::min<uint64_t>((ep.dv / kEmbedDepth + 31) / 32 * 32, kEmbedThreads);
-        ep.tx = (uint32_t)tx;
-        ep.slots = kEmbedThreads / ep.tx;
-        // few rows: a row's columns over several CTAs, one vector a thread
-        const uint64_t groups = (a.n + ep.slots - 1) / ep.slots;
-        const uint64_t most = (ep.dv + ep.tx - 1) / ep.tx;
-        ep.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 2 * kSms / groups));
-        const dim3 grid(grid_of(groups, 8) * ep.split);
-        return wide ? rw_launch(k_embed<TI, TO, ID, kV>, grid, dim3(kEmbedThreads), 0, s, false, a, ep)
-                    : rw_launch(k_embed<TI, TO, ID, 1>, grid, dim3(kEmbedThreads), 0, s, false, a, ep);
-      });
+      using TI = decltype(ti);
+      using TO = decltype(to);
+      constexpr int kV = 16 / sizeof(TI);
+      const bool wide = rw_packs(a.table, a.vocab, a.d, a.ld_table, sizeof(TI), kV) &&
+                        rw_packs(a.out, a.n, a.d, a.ld_out, sizeof(TO), kV);
+      return wide ? embed_launch<TI, TO, kV>(a, s) : embed_launch<TI, TO, 1>(a, s);
     });
   });
 }
@@ -852,15 +887,15 @@ GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
 
 namespace {
 
-ZeroRows zero_rows(const EmbedGradLaunch& a) {
-  const uint64_t elem = rw_type_bytes(a.dtable_type), pitch = a.ld_dtable * elem;
-  ZeroRows z = {(char*)a.dtable, a.vocab, 0, pitch, (uint32_t)elem};
-  uint64_t bytes = a.d * elem;
-  if (a.vocab == 1 || a.ld_dtable == a.d) {  // one run
-    bytes *= a.vocab;
+ZeroRows zero_rows(void* p, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t elem) {
+  const uint64_t pitch = ld * elem;
+  ZeroRows z = {(char*)p, rows, 0, pitch, (uint32_t)elem};
+  uint64_t bytes = cols * elem;
+  if (rows == 1 || ld == cols) {  // one run
+    bytes *= rows;
     z.rows = 1;
   }
-  if (bytes % 16 == 0 && (uintptr_t)a.dtable % 16 == 0 && (z.rows == 1 || pitch % 16 == 0)) z.unit = 16;
+  if (bytes % 16 == 0 && (uintptr_t)p % 16 == 0 && (z.rows == 1 || pitch % 16 == 0)) z.unit = 16;
   z.row_units = bytes / z.unit;
   return z;
 }
@@ -880,7 +915,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   if (a.n == 0) {
     if (a.accumulate) return cudaSuccess;
     *nl += 1;
-    const ZeroRows z = zero_rows(a);
+    const ZeroRows z = zero_rows(a.dtable, a.vocab, a.d, a.ld_dtable, rw_type_bytes(a.dtable_type));
     return rw_launch(k_zero_rows, dim3(zero_ctas(z)), dim3(kCountThreads), 0, s, false, z);
   }
   const GradPlan g = grad_plan(a.n, a.d, a.vocab);
@@ -914,7 +949,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
     e = rw_with_index(a.id_type, [&](auto id) {
       using ID = decltype(id);
       const uint32_t blocks = (uint32_t)((a.n * kCountShare + kCountThreads - 1) / kCountThreads);
-      const ZeroRows z = zero_rows(a);
+      const ZeroRows z = zero_rows(a.dtable, a.vocab, a.d, a.ld_dtable, rw_type_bytes(a.dtable_type));
       return rw_launch(k_token_rank<ID>, dim3(blocks + (zero_first ? zero_ctas(z) : 0)), dim3(kCountThreads),
                        0, s, false, (const ID*)a.ids, (uint32_t)a.n, (uint32_t)a.vocab, buf[0], blocks, z);
     });
@@ -974,6 +1009,10 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
 cudaError_t launch_dropout(const DropoutLaunch& a, cudaStream_t s, int* nl) {
   if (a.rows == 0 || a.cols == 0) return cudaSuccess;
   *nl += 1;
+  if (a.limit >= 65536) {
+    const ZeroRows z = zero_rows(a.y, a.rows, a.cols, a.ld_y, rw_type_bytes(a.type));
+    return rw_launch(k_zero_rows, dim3(zero_ctas(z)), dim3(kCountThreads), 0, s, false, z);
+  }
   const uint64_t groups = (a.rows * a.cols + 7) / 8;
   PhiloxKeys keys;
   for (uint32_t r = 0; r < 10; r++) {
@@ -984,7 +1023,10 @@ cudaError_t launch_dropout(const DropoutLaunch& a, cudaStream_t s, int* nl) {
   const bool vec = flat && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.y % 16 == 0;
   return rw_with_type(a.type, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid(grid_of((groups + 255) / 256, 8)), block(256);
+    constexpr uint64_t kPer = 256 * kDropoutDepth<T>;
+    const uint64_t ctas = (groups + kPer - 1) / kPer;
+    if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
+    const dim3 grid(vec ? (uint32_t)ctas : grid_of((groups + 255) / 256, 8)), block(256);
     return vec ? rw_launch(k_dropout<T, true>, grid, block, 0, s, false, a, keys)
                : rw_launch(k_dropout<T, false>, grid, block, 0, s, false, a, keys);
   });
