@@ -338,7 +338,8 @@ int rw_dropout_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t rows,
                       uint64_t ld_y, void* stream);
 
 /* Log-probabilities of classes from margins x [n][classes], one pass over them. With
- * m = max x of a row and d_j = scale * (x_j - m), scale > 0 (an inverse temperature):
+ * m = max x of a row and d_j = scale * (x_j - m), scale in [1e-20, 1e20] (an inverse
+ * temperature):
  *   row_max m, log_sum log(sum_j e^d_j), lse scale * m + log_sum;
  *   logp     d_t - log_sum of the row's target t; 0 when t is outside 0..classes-1;
  *   entropy  of the row's distribution, in nats;

@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "rw_internal.cuh"
 #include "rw_types.cuh"
@@ -95,6 +96,10 @@ __device__ __forceinline__ RowEnd row_end(const Sums& a) {
   const bool dead = a.m == -kInf;
   return {dead ? 0.0f : a.m, dead ? 0.0f : logf(a.s)};
 }
+// scale * (x - base), of halves: the difference of two margins may be past f32's range.
+__device__ __forceinline__ float scaled_difference(float x, float base, float scale) {
+  return (x * 0.5f - base * 0.5f) * scale * 2.0f;
+}
 template <typename T>
 __device__ __forceinline__ void write_row(const LogprobsLaunch& a, uint64_t i, const Sums& r, const RowEnd& e) {
   if (a.row_max) a.row_max[i] = r.m;
@@ -105,14 +110,14 @@ __device__ __forceinline__ void write_row(const LogprobsLaunch& a, uint64_t i, c
     const int64_t c = a.target_type == RW_I64 ? ((const int64_t*)a.targets)[i] : ((const int32_t*)a.targets)[i];
     float v = 0.0f;
     if (c >= 0 && (uint64_t)c < a.classes)
-      v = (rw_widen(((const T*)a.x)[i * a.ld_x + c]) - e.base) * a.scale - e.log_sum;
+      v = scaled_difference(rw_widen(((const T*)a.x)[i * a.ld_x + c]), e.base, a.scale) - e.log_sum;
     a.logp[i] = v;
   }
 }
 __device__ __forceinline__ void write_top(const LogprobsLaunch& a, uint64_t i, uint32_t place, Key k, const RowEnd& e) {
   if (a.top_index) a.top_index[i * a.top_k + place] = index_of(k);
   if (a.top_logp)
-    a.top_logp[i * a.top_k + place] = (margin_of((uint32_t)(k >> 32)) - e.base) * a.scale - e.log_sum;
+    a.top_logp[i * a.top_k + place] = scaled_difference(margin_of((uint32_t)(k >> 32)), e.base, a.scale) - e.log_sum;
 }
 
 // =================================================================================
@@ -224,6 +229,7 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
 // Many classes: a CTA a row, or a part of one.
 
 constexpr int kRowThreads = 256;
+constexpr int kRowCtas = 4;  // a SM
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
 constexpr uint32_t kGroups = 64;   // groups of threads whose maxima bound the top places
@@ -301,30 +307,29 @@ __device__ __forceinline__ Two pair_of(const Pack<__half, V>& p, int q) {
   return CUT ? two_of(max_nan(f.x, kLowest), max_nan(f.y, kLowest)) : two_of(f.x, f.y);
 }
 
-// The largest of V elements, NaN if one is.
-template <int V>
-__device__ __forceinline__ float pack_max(const Pack<float, V>& p) {
-  float m = p.v[0];
+// The largest element of N packs, NaN if one is.
+template <int N, int V>
+__device__ __forceinline__ float packs_max(const Pack<float, V>* p) {
+  float m = p[0].v[0];
 #pragma unroll
-  for (int k = 1; k < V; k++) m = max_nan(m, p.v[k]);
+  for (int k = 1; k < N * V; k++) m = max_nan(m, p[k / V].v[k % V]);
   return m;
 }
-template <typename T, typename T2, int V>
-__device__ __forceinline__ T2 pair_max(const Pack<T, V>& p) {
-  const T2* w = reinterpret_cast<const T2*>(p.v);
-  T2 m = w[0];
+template <typename T2, int N, typename T, int V>
+__device__ __forceinline__ T2 pairs_max(const Pack<T, V>* p) {
+  T2 m = reinterpret_cast<const T2*>(p[0].v)[0];
 #pragma unroll
-  for (int k = 1; k < V / 2; k++) m = __hmax2_nan(m, w[k]);
+  for (int k = 1; k < N * V / 2; k++) m = __hmax2_nan(m, reinterpret_cast<const T2*>(p[k / (V / 2)].v)[k % (V / 2)]);
   return m;
 }
-template <int V>
-__device__ __forceinline__ float pack_max(const Pack<__nv_bfloat16, V>& p) {
-  const __nv_bfloat162 m = pair_max<__nv_bfloat16, __nv_bfloat162, V>(p);
+template <int N, int V>
+__device__ __forceinline__ float packs_max(const Pack<__nv_bfloat16, V>* p) {
+  const __nv_bfloat162 m = pairs_max<__nv_bfloat162, N>(p);
   return max_nan(__low2float(m), __high2float(m));
 }
-template <int V>
-__device__ __forceinline__ float pack_max(const Pack<__half, V>& p) {
-  const __half2 m = pair_max<__half, __half2, V>(p);
+template <int N, int V>
+__device__ __forceinline__ float packs_max(const Pack<__half, V>* p) {
+  const __half2 m = pairs_max<__half2, N>(p);
   return max_nan(__low2float(m), __high2float(m));
 }
 
@@ -401,7 +406,7 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
       if (v >= sp.vecs) continue;
       Pack<T, kV> p;
       p.load(sp.vec(v));
-      if (order_of(pack_max(p)) < from) continue;
+      if (order_of(packs_max<1>(&p)) < from) continue;
 #pragma unroll
       for (int k = 0; k < kV; k++) offer(p.get(k), sp.head + v * kV + k);
     }
@@ -504,14 +509,15 @@ __device__ __forceinline__ float2 cta_sum(float2 v, float2* s_tmp) {
 // of kRowDepth vectors holds a new maximum.
 //
 // x * c must not overflow: margins below kLowest count as kLowest, and blocks whose maximum
-// so far is not above it are left out. That is exact where the row's maximum is above
-// kLowest; where it is not (a row masked with the type's lowest value), and for scales
-// outside [kScaleLow, kScaleHigh], the sums are taken again as e^{scale (x - m)}.
+// so far is not above it are left out. That is exact where the row's maximum is in range;
+// where it is not (a row masked with the type's lowest value), and for scales far from 1, the
+// sums are taken again as e^{scale (x - m)}.
 // ENT: with the entropy's sum.
-constexpr float kScaleLow = 1e-6f, kScaleHigh = 1e6f;
+__device__ __forceinline__ bool in_range(float m) { return m > kLowest && m < -kLowest; }
+__device__ __forceinline__ bool scale_in_range(float s) { return s >= 1e-6f && s <= 1e6f; }
 
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch a, SplitRow sr) {
+__global__ void __launch_bounds__(kRowThreads, kRowCtas) k_logprobs_row(LogprobsLaunch a, SplitRow sr) {
   __shared__ TopSpace s_top;
   __shared__ float s_max[kRowWarps];
   __shared__ float2 s_sum[kRowWarps];
@@ -526,11 +532,9 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
 
   float m = -kInf, mc = 0.0f;
   Two s = 0, w = 0, c2 = two_of(c, c), base = 0;  // base: -mc twice
-  auto absorb = [&](const Pack<T, kV>* p, int count) {  // count: a constant after unrolling
-    float top = pack_max(p[0]);
-#pragma unroll
-    for (int u = 1; u < kRowDepth; u++)
-      if (u < count) top = max_nan(top, pack_max(p[u]));
+  auto absorb = [&](const Pack<T, kV>* p, auto packs) {
+    constexpr int kCount = decltype(packs)::value;
+    float top = packs_max<kCount>(p);
     if (!(top <= m)) {
       top = max_nan(top, m);
       const float next = top * c;
@@ -546,8 +550,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
     }
     if (m <= kLowest) return;
 #pragma unroll
-    for (int u = 0; u < kRowDepth; u++) {
-      if (u >= count) break;
+    for (int u = 0; u < kCount; u++) {
 #pragma unroll
       for (int q = 0; q < kV / 2; q++) {
         const Two d = fma2(pair_of<ENT>(p[u], q), c2, base);
@@ -558,6 +561,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
       }
     }
   };
+  const std::integral_constant<int, kRowDepth> kBlockPacks;
+  const std::integral_constant<int, 1> kOnePack;
   // a block is summed while the next one's loads are in flight
   constexpr uint32_t kBlock = kRowDepth * kRowThreads;
   uint32_t v = t;
@@ -572,24 +577,24 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
     for (;;) {
       v += kBlock;
       if (!whole(v)) {
-        absorb(p[0], kRowDepth);
+        absorb(p[0], kBlockPacks);
         break;
       }
       fetch(p[1], v);
-      absorb(p[0], kRowDepth);
+      absorb(p[0], kBlockPacks);
       v += kBlock;
       if (!whole(v)) {
-        absorb(p[1], kRowDepth);
+        absorb(p[1], kBlockPacks);
         break;
       }
       fetch(p[0], v);
-      absorb(p[1], kRowDepth);
+      absorb(p[1], kBlockPacks);
     }
   }
   for (; v < sp.vecs; v += kRowThreads) {
     Pack<T, kV> p;
     p.load(sp.vec(v));
-    absorb(&p, 1);
+    absorb(&p, kOnePack);
   }
   Sums r;
   r.m = m;
@@ -611,7 +616,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_logprobs_row(LogprobsLaunch 
   const float all = cta_max(own, s_max);
   if (a.top_k) top_groups(s_top);
   if (all != -kInf) {
-    if ((all <= kLowest) || !(a.scale >= kScaleLow && a.scale <= kScaleHigh)) {
+    if (!(in_range(all) && scale_in_range(a.scale))) {
       r.s = r.t = 0.0f;
       for (uint32_t j = t; j < sp.n; j += kRowThreads) {
         const float d = max_nan(rw_widen(sp.x[j]) - all, kLowest), e = exp2_fast(d * c);
@@ -735,8 +740,7 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobsGradLaunch& a, uint64_
   }
   const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f;
   if (g == 0.0f && e == 0.0f) return r;
-  // the constants would overflow below kLowest and for scales far from 1
-  if (m <= kLowest || !(a.scale >= kScaleLow && a.scale <= kScaleHigh)) {
+  if (!(in_range(m) && scale_in_range(a.scale))) {  // the constants could overflow
     r.kind = 2;
     return r;
   }

@@ -813,6 +813,7 @@ struct DeviceScope {
 };
 
 constexpr uint64_t kMaxItems = (1ull << 31) - 1;
+bool scale_ok(float s) { return s >= 1e-20f && s <= 1e20f; }
 constexpr uint64_t kMaxWidth = (1ull << 23) - 1;
 
 bool elem_type_ok(int32_t t) { return t == RW_F32 || t == RW_BF16 || t == RW_F16; }
@@ -979,7 +980,7 @@ extern "C" int rw_logprobs_device(rw_ctx* ctx, const void* d_x, int32_t type, ui
       [&]() -> std::string {
         if (!elem_type_ok(type)) return "unknown element type";
         if (!index_type_ok(target_type)) return "unknown target type";
-        if (!(scale > 0.0f && scale <= 3.0e38f)) return "scale is not positive and finite";
+        if (!scale_ok(scale)) return "scale is not in [1e-20, 1e20]";
         if (classes > kMaxItems) return "classes must be below 2^31";
         if (top_k > RW_MAX_TOP || top_k > classes) return "top_k is above RW_MAX_TOP or classes";
         RW_MATRIX(d_x, n, classes, ld_x, elem_bytes(type));
@@ -1024,7 +1025,7 @@ extern "C" int rw_logprobs_grad_device(rw_ctx* ctx, const void* d_x, int32_t typ
       [&]() -> std::string {
         if (!elem_type_ok(type)) return "unknown element type";
         if (!index_type_ok(target_type)) return "unknown target type";
-        if (!(scale > 0.0f && scale <= 3.0e38f)) return "scale is not positive and finite";
+        if (!scale_ok(scale)) return "scale is not in [1e-20, 1e20]";
         if (classes > kMaxItems) return "classes must be below 2^31";
         if (n == 0 || classes == 0) return "";
         RW_MATRIX(d_x, n, classes, ld_x, elem_bytes(type));

@@ -375,6 +375,59 @@ def test_logprobs_masks_and_ties(ctx, v, dtype):
             check_logprobs(tokens.logprobs(ctx, strided(x), t, scale=scale, top_k=k), x, t, scale, k)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_logprobs_largest_margins_side_by_side(ctx, dtype):
+    """The largest margins lie 8 (4) at a time every 256 vectors, all in few threads' shares."""
+    v = 140000
+    x, t = margins(1, 3, v, dtype)
+    per = 16 // x.element_size()
+    at = torch.arange(v, device="cuda")
+    share = (at // per) % 256
+    for row, threads in ((0, 4), (1, 9), (2, 31)):
+        x[row] += torch.where(share < threads, 30.0, 0.0).to(dtype)
+    for k in (1, 5, 32):
+        check_logprobs(tokens.logprobs(ctx, x, t, top_k=k), x, t, 1.0, k)
+        one = tokens.logprobs(ctx, x[:1].repeat(600, 1), t[:1].repeat(600), top_k=k)  # rows not split
+        assert torch.equal(one.top_index, tokens.logprobs(ctx, x[:1], t[:1], top_k=k).top_index.expand(600, k))
+
+
+@pytest.mark.parametrize("v", [7, 100, 900, 1500, 30000])
+def test_logprobs_far_margins_and_scales(ctx, v):
+    """Margins near the ends of f32's range, a shared offset, and scales far from 1."""
+    x, t = margins(v, 5, v, F32)
+    x[1] *= 5e37
+    x[2] += 4096.0
+    x[3] = -3e38
+    x[3, v // 2] = -2.9e38
+    x[4] *= 1e-12
+    x, t = torch.cat([x, x[:1] * 2e37]), torch.cat([t, t[:1]])
+    # beyond 900 classes some margins of row 1 are above 3.4e38 / 5e37 and so +inf
+    over = x.isposinf().any(1)
+    for scale in (1.0, 1e-19, 1e-7, 1e7, 1e19):
+        r = tokens.logprobs(ctx, x, t, scale=scale, top_k=2)
+        assert r.log_sum[over].isnan().all() and r.entropy[over].isnan().all()
+        r = type(r)(*(f[~over] for f in r))
+        check_far_margins(ctx, x[~over], t[~over], scale, v, r)
+
+
+def check_far_margins(ctx, x, t, scale, v, r):
+    m, log_sum, _, logp, ent, _, order, _ = logprob_reference(x, t, scale, 2)
+    # d = scale (x - m) is off by |d| 2^-23: the sum's terms by |d| e^d 2^-23, and |d| e^d
+    # is below 0.37, so the sum of at most v of them is off by v * 0.37 * 2^-23 at most
+    tol = (v * 0.74 + 64 + v / 128) * U
+    assert torch.equal(r.top_index, order)
+    assert ((r.log_sum.double() - log_sum).abs() <= tol + U * log_sum).all()
+    big = logp.abs() * 4 * U + tol
+    f32_range = logp.abs() < 3e38  # beyond it, -inf
+    assert ((r.logp.double() - logp).abs() <= big)[f32_range].all()
+    assert (r.logp[~f32_range] == -INF).all()
+    # the terms d e^d: their size times their own relative error, |d| 2^-22 and less
+    assert ((r.entropy.double() - ent).abs() <= 4 * tol + 8 * U * ent).all()
+    g, e = -torch.ones(len(x), device="cuda"), torch.full((len(x),), 0.5, device="cuda")
+    got = tokens.logprobs_grad(ctx, x, t, r.row_max, r.log_sum, r.entropy, g, e, scale=scale)
+    check_logprobs_grad(got, x, t, r.row_max, r.log_sum, r.entropy, g, e, scale)
+
+
 @pytest.mark.parametrize("v", [5, 30, 700, 5000, 140000])
 def test_logprobs_of_nan_and_infinity(ctx, v):
     x, t = margins(v, 5, v, F32)
@@ -651,3 +704,73 @@ def test_own_stream_of_the_context(ctx):
                                       y.data_ptr(), 8, s))
     torch.cuda.synchronize()
     assert torch.equal(y, tokens.dropout(ctx, x, 0.5, 1, 2))
+
+
+def guarded(bytes_needed):
+    """A workspace of exactly that many bytes, of all ones, between bytes that must stay."""
+    buf = torch.full((bytes_needed + 512,), 255, device="cuda", dtype=torch.uint8)
+    return buf, buf[256:256 + bytes_needed], (lambda: bool((buf[:256] == 255).all() and (buf[256 + bytes_needed:] == 255).all()))
+
+
+@pytest.mark.parametrize("n,d,vocab", [(700, 33, 40), (700, 40, 2000), (30000, 33, 40), (30000, 33, 4000),
+                                       (30000, 128, 300), (9, 3, 2)])
+def test_embed_grad_workspace_contents_do_not_matter(ctx, n, d, vocab):
+    """Through the C entry point: any contents, no byte outside it, no byte between rows."""
+    import ctypes as C
+    ids, grad = rand_ids(n, n, vocab), rand(n, n, d)
+    want = tokens.embed_grad(ctx, grad, ids, vocab)
+    need = C.c_uint64()
+    ctx.check(N.lib.rw_embed_grad_workspace(ctx.h, n, d, vocab, C.byref(need)))
+    buf, ws, fine = guarded(need.value)
+    out = torch.full((vocab, d + 5), 3.0, device="cuda")
+    ctx.check(N.lib.rw_embed_grad_device(ctx.h, grad.data_ptr(), N.RW_F32, d, ids.data_ptr(), N.RW_I64, n, d,
+                                         vocab, 1.0, 0, out.data_ptr(), N.RW_F32, d + 5, ws.data_ptr(),
+                                         need.value, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out[:, :d], want) and (out[:, d:] == 3).all() and fine()
+
+
+@pytest.mark.parametrize("n,v", [(1, 128000), (8, 50001), (100, 20000), (3, 9000)])
+def test_logprobs_workspace_contents_do_not_matter(ctx, n, v):
+    import ctypes as C
+    x, t = margins(v, n, v, BF16)
+    want = tokens.logprobs(ctx, x, t, top_k=32)
+    need = C.c_uint64()
+    ctx.check(N.lib.rw_logprobs_workspace(ctx.h, n, v, N.RW_BF16, 32, C.byref(need)))
+    assert need.value > 0
+    buf, ws, fine = guarded(need.value)
+    row = torch.full((5, n), 3.0, device="cuda")
+    top, index = torch.full((n, 32), 3.0, device="cuda"), torch.full((n, 32), 3, device="cuda")
+    ctx.check(N.lib.rw_logprobs_device(ctx.h, x.data_ptr(), N.RW_BF16, n, v, v, 1.0, t.data_ptr(), N.RW_I64, 32,
+                                       *(r.data_ptr() for r in row), top.data_ptr(), index.data_ptr(),
+                                       ws.data_ptr(), need.value, torch.cuda.current_stream().cuda_stream))
+    assert all(torch.equal(a, b) for a, b in zip((*row, top, index), want)) and fine()
+
+
+@pytest.mark.parametrize("v", [7, 2000])
+def test_logprobs_outputs_may_be_left_out(ctx, v):
+    x, t = margins(v, 40, v, F32)
+    want = tokens.logprobs(ctx, x, t, top_k=3)
+    s = torch.cuda.current_stream().cuda_stream
+    need = 1 << 20
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    full = [want.row_max, want.log_sum, want.lse, want.logp, want.entropy, want.top_logp, want.top_index]
+    for keep in range(7):
+        outs = [torch.empty_like(f) if i == keep else None for i, f in enumerate(full)]
+        ctx.check(N.lib.rw_logprobs_device(ctx.h, x.data_ptr(), N.RW_F32, 40, v, v, 1.0,
+                                           t.data_ptr() if keep == 3 else None, N.RW_I64, 3,
+                                           *(None if o is None else o.data_ptr() for o in outs),
+                                           ws.data_ptr(), need, s))
+        # without the entropy's sum the exponentials are the same; only summation order may not be
+        assert torch.allclose(outs[keep].double(), full[keep].double(), rtol=1e-6, atol=1e-6)
+
+
+def test_strided_outputs_keep_what_lies_between(ctx):
+    x = rand(1, 50, 3000)
+    t = torch.zeros(50, dtype=torch.int64, device="cuda")
+    r = tokens.logprobs(ctx, x, t)
+    for call in (lambda o: tokens.dropout(ctx, x, 0.5, 1, out=o),
+                 lambda o: tokens.logprobs_grad(ctx, x, t, r.row_max, r.log_sum, None, -r.lse, out=o),
+                 lambda o: tokens.dropout(ctx, x, 1.0, 1, out=o)):
+        buf = torch.full((50, 3011), 7.0, device="cuda")
+        call(buf[:, 5:3005])
+        assert (buf[:, :5] == 7).all() and (buf[:, 3005:] == 7).all()

@@ -90,6 +90,8 @@ CASES = [
     (logprobs, dict(scale=-1.0), "scale"),
     (logprobs, dict(scale=NAN), "scale"),
     (logprobs, dict(scale=INF), "scale"),
+    (logprobs, dict(scale=1e-30), "scale"),
+    (logprobs, dict(scale=1e30), "scale"),
     (logprobs, dict(classes=1 << 31, ld_x=1 << 31), "below 2^31"),
     (logprobs, dict(top_k=9), "top_k"),
     (logprobs, dict(top_k=33, classes=100, ld_x=100), "top_k"),
