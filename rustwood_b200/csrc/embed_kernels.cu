@@ -66,13 +66,8 @@ __global__ void __launch_bounds__(kEmbedThreads) k_embed(EmbedLaunch a, EmbedPla
       for (int u = 0; u < C; u++) {
         if (c + u * step >= ep.dv) break;
         Pack<TO, V> o;
-        if (id[r] >= 0) {
 #pragma unroll
-          for (int k = 0; k < V; k++) o.set(k, a.scale * v[r][u].get(k));
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; k++) o.set(k, 0.0f);
-        }
+        for (int k = 0; k < V; k++) o.set(k, id[r] >= 0 ? a.scale * v[r][u].get(k) : 0.0f);
         o.store_streaming(out + (c + u * step) * V);
       }
     }
@@ -284,6 +279,7 @@ struct ChunkPlan {
   uint32_t sum_ctas;    // CTAs that sum; the rest zero rows that no id names
   uint64_t dv;          // vectors a row
   uint64_t pitch;       // floats of one partial row (a multiple of 4)
+  uint32_t join_lanes;  // lanes of k_embed_join for a row: a power of two
 };
 
 __device__ __forceinline__ uint32_t key_of(unsigned long long pair) { return (uint32_t)(pair >> 32); }
@@ -386,7 +382,8 @@ __global__ void __launch_bounds__(kSumThreads)
 
 // Adds the partial sums of the runs that cross chunks: CTA (x, y) takes the runs that start
 // in chunks x, x + gridDim.x, .. and the columns of block y. A run of a few chunks is one
-// warp's, a longer one is shared by all warps and their sums are added in order.
+// warp's, a longer one is shared by all warps and their sums are added in order. Where a row
+// has fewer than 32 float4s, groups of lanes take every 2nd, 4th, .. chunk.
 template <typename TD>
 __global__ void __launch_bounds__(kJoinThreads)
     k_embed_join(EmbedGradLaunch a, ChunkPlan cp, const unsigned long long* __restrict__ pairs,
@@ -397,7 +394,8 @@ __global__ void __launch_bounds__(kJoinThreads)
   __shared__ uint32_t s_count;
   __shared__ float4 s_part[kWarps][32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t col = (uint64_t)blockIdx.y * kJoinCols + lane * 4;
+  const uint32_t width = cp.join_lanes, groups = 32 / width, group = lane / width;
+  const uint64_t col = (uint64_t)blockIdx.y * kJoinCols + lane % width * 4;
   TD* dtable = (TD*)a.dtable;
   rw_dependent_start();
 
@@ -406,7 +404,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (col < cp.pitch) {
 #pragma unroll 8
-      for (uint32_t q = lo; q < hi; q++) {
+      for (uint32_t q = lo + group; q < hi; q += groups) {
         const float4 v = *(const float4*)(partial + ((uint64_t)q * 2 + (q == first ? 1 : 0)) * cp.pitch + col);
         s.x += v.x;
         s.y += v.y;
@@ -414,9 +412,16 @@ __global__ void __launch_bounds__(kJoinThreads)
         s.w += v.w;
       }
     }
+    for (uint32_t o = width; o < 32; o *= 2) {
+      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+      s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+      s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+    }
     return s;
   };
   auto finish = [&](uint32_t first, float4 s) {
+    if (group != 0) return;
     const uint64_t end = min((uint64_t)(first + 1) * cp.chunk, a.n);
     TD* p = dtable + (uint64_t)key_of(pairs[end - 1]) * a.ld_dtable + col;
     const float v[4] = {s.x, s.y, s.z, s.w};
@@ -826,6 +831,8 @@ ChunkPlan chunk_plan(uint64_t n, uint64_t d, int V) {
   c.slots = kSumThreads / c.tx;
   c.col_blocks = (uint32_t)((c.dv + c.tx - 1) / c.tx);
   c.pitch = (d + 3) / 4 * 4;
+  c.join_lanes = 1;
+  while (c.join_lanes < 32 && c.join_lanes * 4 < d) c.join_lanes *= 2;
   const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * (c.tx >= 64 ? 16 : 4) * c.slots / c.col_blocks);
   const uint64_t most = std::min<uint64_t>(want, 32768);
   c.chunk = (uint32_t)std::max<uint64_t>(8, (n + most - 1) / most);

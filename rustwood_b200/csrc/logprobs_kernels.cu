@@ -124,6 +124,7 @@ __device__ __forceinline__ void write_top(const LogprobsLaunch& a, uint64_t i, u
 // Few classes: L lanes a row, at most E margins a lane, all in registers.
 
 constexpr int kGroupThreads = 256;
+constexpr uint32_t kCountPlaces = 6;
 constexpr int kGroupCand = 128;  // candidates for a row's top places that a warp keeps
 
 template <typename T, int L, int E>
@@ -178,24 +179,44 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
       const uint32_t who = __ballot_sync(0xffffffffu, above == a.top_k - 1);
       const uint32_t bound = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
       Key* cand = s_cand[threadIdx.x / 32];
-      uint32_t count = 0;
-      __syncwarp();
+      auto collect = [&](uint32_t from) {
+        uint32_t count = 0;
+        __syncwarp();
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const uint32_t o = order_of(v[e]);
-        const bool in = o >= bound && lane + e * 32 < classes;
-        const uint32_t hits = __ballot_sync(0xffffffffu, in);
-        const uint32_t at = count + __popc(hits & ((1u << lane) - 1));
-        if (in && at < kGroupCand) cand[at] = key_of(o, lane + e * 32);
-        count += __popc(hits);
+        for (int e = 0; e < E; e++) {
+          const uint32_t o = order_of(v[e]);
+          const bool in = o >= from && lane + e * 32 < classes;
+          const uint32_t hits = __ballot_sync(0xffffffffu, in);
+          const uint32_t at = count + __popc(hits & ((1u << lane) - 1));
+          if (in && at < kGroupCand) cand[at] = key_of(o, lane + e * 32);
+          count += __popc(hits);
+        }
+        __syncwarp();
+        return count;
+      };
+      uint32_t count = collect(bound), ties = 0;
+      if (count > kGroupCand && bound != 0xffffffffu) {
+        // many equal the bound (a mask): those above it, then the first of the equal ones
+        count = collect(bound + 1);
+        ties = count < a.top_k ? a.top_k - count : 0;
       }
-      __syncwarp();
       if (count <= kGroupCand) {
         for (uint32_t q = lane; q < count; q += 32) {
           const Key k = cand[q];
           uint32_t place = 0;
+#pragma unroll 4
           for (uint32_t w = 0; w < count; w++) place += cand[w] > k;
           if (real && place < a.top_k) write_top(a, i, place, k, end);
+        }
+        uint32_t place = a.top_k - ties;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          if (place >= a.top_k) break;
+          const bool in = order_of(v[e]) == bound && lane + e * 32 < classes;
+          const uint32_t hits = __ballot_sync(0xffffffffu, in);
+          const uint32_t at = place + __popc(hits & ((1u << lane) - 1));
+          if (real && in && at < a.top_k) write_top(a, i, at, key_of(bound, lane + e * 32), end);
+          place += __popc(hits);
         }
         continue;
       }
@@ -204,6 +225,31 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
     uint32_t order[E];
 #pragma unroll
     for (int e = 0; e < E; e++) order[e] = lane + e * L < classes ? order_of(v[e]) : 0;
+    if constexpr (L * E <= 32) {
+      // many places of few margins: every margin counts those before it
+      if (a.top_k > kCountPlaces) {
+        uint32_t above[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) above[e] = 0;
+#pragma unroll
+        for (int o = 0; o < L; o++) {
+#pragma unroll
+          for (int q = 0; q < E; q++) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, order[q], o);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+              const bool lower = q < e || (q == e && (lane ^ o) < lane);
+              above[e] += other > order[e] || (other == order[e] && lower);
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (real && order[e] && above[e] < a.top_k)
+            write_top(a, i, above[e], key_of(order[e], lane + e * L), end);
+        continue;
+      }
+    }
     for (uint32_t place = 0; place < a.top_k; place++) {
       uint32_t top = order[0], at = lane;
 #pragma unroll
@@ -228,15 +274,13 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
 // =================================================================================
 // Many classes: a CTA a row, or a part of one.
 
-constexpr int kRowThreads = 256;
-constexpr int kRowCtas = 4;  // a SM
-constexpr int kRowWarps = kRowThreads / 32;
+// Threads a CTA: 256, or 64 for many short rows, whose barriers and joins cost more than
+// their margins (48056 x 2824 bf16: 344 -> XX us).
+constexpr int kRowThreads = 256, kShortThreads = 64;
+constexpr uint64_t kShortBytes = 32 << 10;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
 constexpr uint32_t kGroups = 64;   // groups of threads whose maxima bound the top places
 constexpr uint32_t kCand = 1024;   // candidates for the top places that a CTA keeps
-// Threads that hold a margin above the bound are fewer than top_k groups'. With more that
-// reach it, many margins equal it.
-constexpr uint32_t kLook = kMaxTop * (kRowThreads / kGroups);
 constexpr uint32_t kMaxParts = 64;
 
 // Where a row's sums and top keys are left when it is split: [row][part].
@@ -333,12 +377,18 @@ __device__ __forceinline__ float packs_max(const Pack<__half, V>* p) {
   return max_nan(__low2float(m), __high2float(m));
 }
 
+template <int NT>
 struct TopSpace {
-  uint32_t order[kRowThreads];  // each thread's largest
+  static constexpr int kWarps = NT / 32;
+  static constexpr uint32_t kGroupSize = NT / kGroups;
+  // Threads that hold a margin above the bound are fewer than top_k groups'. With more that
+  // reach it, many margins equal it.
+  static constexpr uint32_t kLook = kMaxTop * kGroupSize;
+  uint32_t order[NT];  // each thread's largest
   uint32_t group[kGroups];
   Key cand[kCand];
-  uint32_t warp[kRowWarps];
-  Key warp_key[kRowWarps];
+  uint32_t warp[kWarps];
+  Key warp_key[kWarps];
   uint32_t look[kLook];
   uint32_t count, bound, looking;
 };
@@ -346,25 +396,28 @@ struct TopSpace {
 // The first two steps of top_places, each followed by a barrier of the caller's: every
 // thread's largest margin, and the groups' largest. The threads of a group are far apart, so
 // neighbours in a row fall into different groups.
-constexpr uint32_t kGroupSize = kRowThreads / kGroups;
-__device__ __forceinline__ void top_threads(float own, TopSpace& s) {
+template <int NT>
+__device__ __forceinline__ void top_threads(float own, TopSpace<NT>& s) {
   s.order[threadIdx.x] = order_of(own);
   if (threadIdx.x == 0) s.count = s.looking = 0;
 }
-__device__ __forceinline__ void top_groups(TopSpace& s) {
+template <int NT>
+__device__ __forceinline__ void top_groups(TopSpace<NT>& s) {
   const uint32_t t = threadIdx.x;
   if (t < kGroups) {
     uint32_t g = s.order[t];
 #pragma unroll
-    for (uint32_t q = 1; q < kGroupSize; q++) g = max(g, s.order[t + q * kGroups]);
+    for (uint32_t q = 1; q < TopSpace<NT>::kGroupSize; q++) g = max(g, s.order[t + q * kGroups]);
     s.group[t] = g;
   }
 }
 
 // The top_k places among the span's margins, in order, after top_threads and top_groups;
 // emit(place, key) is called once a place. All threads of the CTA call it.
-template <typename T, typename Emit>
-__device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32_t top_k, TopSpace& s, Emit emit) {
+template <typename T, int NT, typename Emit>
+__device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32_t top_k, TopSpace<NT>& s, Emit emit) {
+  constexpr int kRowThreads = NT, kRowWarps = NT / 32;
+  constexpr uint32_t kGroupSize = TopSpace<NT>::kGroupSize, kLook = TopSpace<NT>::kLook;
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   constexpr int kV = Span<T>::kV;
   const uint32_t mine = order_of(own);
@@ -476,17 +529,19 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
 }
 
 // The whole CTA's maximum, and its sum of v.x and v.y, in a fixed order.
-__device__ __forceinline__ float cta_max(float m, float* s_tmp) {
+template <int W>
+__device__ __forceinline__ float cta_max(float m, float (&s_tmp)[W]) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) s_tmp[threadIdx.x >> 5] = m;
   __syncthreads();
   m = s_tmp[0];
 #pragma unroll
-  for (int w = 1; w < kRowWarps; w++) m = max_nan(m, s_tmp[w]);
+  for (int w = 1; w < W; w++) m = max_nan(m, s_tmp[w]);
   return m;
 }
-__device__ __forceinline__ float2 cta_sum(float2 v, float2* s_tmp) {
+template <int W>
+__device__ __forceinline__ float2 cta_sum(float2 v, float2 (&s_tmp)[W]) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
@@ -496,7 +551,7 @@ __device__ __forceinline__ float2 cta_sum(float2 v, float2* s_tmp) {
   __syncthreads();
   v = s_tmp[0];
 #pragma unroll
-  for (int w = 1; w < kRowWarps; w++) {
+  for (int w = 1; w < W; w++) {
     v.x += s_tmp[w].x;
     v.y += s_tmp[w].y;
   }
@@ -516,9 +571,10 @@ __device__ __forceinline__ float2 cta_sum(float2 v, float2* s_tmp) {
 __device__ __forceinline__ bool in_range(float m) { return m > kLowest && m < -kLowest; }
 __device__ __forceinline__ bool scale_in_range(float s) { return s >= 1e-6f && s <= 1e6f; }
 
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(kRowThreads, kRowCtas) k_logprobs_row(LogprobsLaunch a, SplitRow sr) {
-  __shared__ TopSpace s_top;
+template <typename T, bool ENT, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a, SplitRow sr) {
+  constexpr int kRowThreads = NT, kRowWarps = NT / 32;
+  __shared__ TopSpace<NT> s_top;
   __shared__ float s_max[kRowWarps];
   __shared__ float2 s_sum[kRowWarps];
   constexpr int kV = Span<T>::kV;
@@ -929,7 +985,9 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
       };
       if (a.classes <= 8) return go(k_logprobs_few<T, 1, 8>, 1);
       if (a.classes <= 32) return go(k_logprobs_few<T, 4, 8>, 4);
-      if (a.classes <= 128) return go(k_logprobs_few<T, 8, 16>, 8);
+      // four rows a warp; many places are found faster with a warp a row
+      if (a.classes <= 128)
+        return a.top_k <= 4 ? go(k_logprobs_few<T, 8, 16>, 8) : go(k_logprobs_few<T, 32, 4>, 32);
       if (a.classes <= 256) return go(k_logprobs_few<T, 32, 8>, 32);
       if (a.classes <= 512) return go(k_logprobs_few<T, 32, 16>, 32);
       return go(k_logprobs_few<T, 32, 32>, 32);
@@ -941,9 +999,14 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
   r.keys = (Key*)((char*)workspace + (cells * sizeof(Sums) + 255) / 256 * 256);
   return rw_with_type(a.type, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid((uint32_t)cells), block(kRowThreads);
-    cudaError_t e = a.entropy ? rw_launch(k_logprobs_row<T, true>, grid, block, 0, s, false, a, r)
-                              : rw_launch(k_logprobs_row<T, false>, grid, block, 0, s, false, a, r);
+    const dim3 grid((uint32_t)cells);
+    const bool narrow = a.n >= 148 * 4 && a.classes * sizeof(T) <= kShortBytes;
+    auto go = [&](auto* k, int threads) { return rw_launch(k, grid, dim3(threads), 0, s, false, a, r); };
+    cudaError_t e;
+    if (narrow) e = a.entropy ? go(k_logprobs_row<T, true, kShortThreads>, kShortThreads)
+                              : go(k_logprobs_row<T, false, kShortThreads>, kShortThreads);
+    else e = a.entropy ? go(k_logprobs_row<T, true, kRowThreads>, kRowThreads)
+                       : go(k_logprobs_row<T, false, kRowThreads>, kRowThreads);
     if (e != cudaSuccess || r.parts == 1) return e;
     *nl += 1;
     return rw_launch(k_logprobs_join<T>, dim3((uint32_t)a.n), dim3(kJoinThreads), 0, s, true, a, r);
