@@ -310,7 +310,7 @@ enum { RW_I32 = 0, RW_I64 = 1 };
 
 /* Embedding lookup: out[i] = scale * table[ids[i]], n rows of d, the product in f32 and
  * rounded once to out_type. An id outside 0..vocab-1 (padding, an unseen category) gives a
- * row of zeros. */
+ * row of zeros. d < 2^23. */
 int rw_embed_device(rw_ctx* ctx, const void* d_table, int32_t table_type, uint64_t vocab,
                     uint64_t ld_table, const void* d_ids, int32_t id_type, uint64_t n, uint64_t d,
                     float scale, void* d_out, int32_t out_type, uint64_t ld_out, void* stream);

@@ -29,7 +29,7 @@ constexpr int kEmbedThreads = 256;
 
 struct EmbedPlan {
   uint32_t tx, slots;
-  uint64_t dv;     // vectors a row
+  uint32_t dv;     // vectors a row
   uint32_t split;  // CTAs that share a row's columns
 };
 
@@ -37,8 +37,8 @@ template <typename TI, typename TO, int V, int R, int C>
 __global__ void __launch_bounds__(kEmbedThreads) k_embed(EmbedLaunch a, EmbedPlan ep) {
   const uint32_t slot = threadIdx.x / ep.tx, lane = threadIdx.x % ep.tx;
   if (slot >= ep.slots) return;
-  const uint64_t step = (uint64_t)ep.tx * ep.split;
-  const uint64_t first = (uint64_t)(blockIdx.x % ep.split) * ep.tx + lane;
+  const uint32_t step = ep.tx * ep.split;
+  const uint32_t first = blockIdx.x % ep.split * ep.tx + lane;
   const uint64_t i0 = (uint64_t)(blockIdx.x / ep.split) * ep.slots * R + slot;
   int64_t id[R];
 #pragma unroll
@@ -48,14 +48,14 @@ __global__ void __launch_bounds__(kEmbedThreads) k_embed(EmbedLaunch a, EmbedPla
     if (i < a.n) id[r] = a.id_type == RW_I64 ? ((const int64_t*)a.ids)[i] : ((const int32_t*)a.ids)[i];
     if (id[r] >= 0 && (uint64_t)id[r] >= a.vocab) id[r] = -1;
   }
-  for (uint64_t c = first; c < ep.dv; c += step * C) {
+  for (uint32_t c = first; c < ep.dv; c += step * C) {
     Pack<TI, V> v[R][C];
 #pragma unroll
     for (int r = 0; r < R; r++) {
       const TI* row = (const TI*)a.table + (uint64_t)max(id[r], (int64_t)0) * a.ld_table;
 #pragma unroll
       for (int u = 0; u < C; u++)
-        if (id[r] >= 0 && c + u * step < ep.dv) v[r][u].load(row + (c + u * step) * V);
+        if (id[r] >= 0 && c + u * step < ep.dv) v[r][u].load(row + (uint64_t)(c + u * step) * V);
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kEmbedThreads) k_embed(EmbedLaunch a, EmbedPla
         Pack<TO, V> o;
 #pragma unroll
         for (int k = 0; k < V; k++) o.set(k, id[r] >= 0 ? a.scale * v[r][u].get(k) : 0.0f);
-        o.store_streaming(out + (c + u * step) * V);
+        o.store_streaming(out + (uint64_t)(c + u * step) * V);
       }
     }
   }
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kCountThreads)
 
 constexpr int kSumThreads = 256;
 constexpr int kSumDepth = 4;    // rows in flight per thread
-constexpr int kZeroRows = 64;   // table rows a zeroing CTA covers
+constexpr int kZeroRows = 128;  // the most table rows a zeroing CTA covers
 constexpr int kJoinThreads = 512;
 constexpr int kJoinCols = 128;  // columns of one join (a float4 a lane)
 constexpr uint32_t kNone = 0xffffffffu;
@@ -279,6 +279,7 @@ struct ChunkPlan {
   uint32_t sum_ctas;    // CTAs that sum; the rest zero rows that no id names
   uint64_t dv;          // vectors a row
   uint64_t pitch;       // floats of one partial row (a multiple of 4)
+  uint32_t zero_rows;   // table rows a zeroing CTA covers
   uint32_t join_lanes;  // lanes of k_embed_join for a row: a power of two
 };
 
@@ -304,8 +305,8 @@ __global__ void __launch_bounds__(kSumThreads)
   rw_dependent_start();
   if (blockIdx.x >= cp.sum_ctas) {  // zero the rows of this block that no id names
     __shared__ bool s_absent[kZeroRows];
-    const uint64_t first = (uint64_t)(blockIdx.x - cp.sum_ctas) * kZeroRows;
-    if (threadIdx.x < kZeroRows && first + threadIdx.x < a.vocab) {
+    const uint64_t first = (uint64_t)(blockIdx.x - cp.sum_ctas) * cp.zero_rows;
+    if (threadIdx.x < cp.zero_rows && first + threadIdx.x < a.vocab) {
       const uint32_t key = (uint32_t)(first + threadIdx.x);
       const uint64_t at = lower_bound(pairs, a.n, key);
       s_absent[threadIdx.x] = at == a.n || key_of(pairs[at]) != key;
@@ -315,10 +316,10 @@ __global__ void __launch_bounds__(kSumThreads)
     Pack<TD, V> zero;
 #pragma unroll
     for (int k = 0; k < V; k++) zero.set(k, 0.0f);
-    for (uint64_t r = slot; r < kZeroRows && first + r < a.vocab; r += cp.slots) {
+    for (uint64_t r = slot; r < cp.zero_rows && first + r < a.vocab; r += cp.slots) {
       if (!s_absent[r]) continue;
       TD* row = dtable + (first + r) * a.ld_dtable;
-      for (uint64_t c = lane; c < cp.dv; c += cp.tx) zero.store(row + c * V);
+      for (uint64_t c = lane; c < cp.dv; c += cp.tx) zero.store_streaming(row + c * V);
     }
     return;
   }
@@ -772,11 +773,11 @@ namespace {
 template <typename TI, typename TO, int V>
 cudaError_t embed_launch(const EmbedLaunch& a, cudaStream_t s) {
   EmbedPlan ep;
-  ep.dv = a.d / V;
+  ep.dv = (uint32_t)(a.d / V);
   // few rows: a vector a thread, a row's columns over several CTAs; many: four a thread, of one
   // row where a row has four warps' worth, else of two or four rows
   const bool many = a.n >= 8 * kSms;
-  const uint64_t warps = (ep.dv + 31) / 32;
+  const uint32_t warps = (ep.dv + 31) / 32;
   const int c = !many ? 1 : warps >= 4 ? 4 : warps >= 2 ? 2 : 1, r = many ? 4 / c : 1;
   uint64_t tx = ep.dv;
   if (c > 1) tx = ((ep.dv + c - 1) / c + 31) / 32 * 32;
@@ -803,9 +804,12 @@ cudaError_t launch_embed(const EmbedLaunch& a, cudaStream_t s, int* nl) {
       using TI = decltype(ti);
       using TO = decltype(to);
       constexpr int kV = 16 / sizeof(TI);
-      const bool wide = rw_packs(a.table, a.vocab, a.d, a.ld_table, sizeof(TI), kV) &&
-                        rw_packs(a.out, a.n, a.d, a.ld_out, sizeof(TO), kV);
-      return wide ? embed_launch<TI, TO, kV>(a, s) : embed_launch<TI, TO, 1>(a, s);
+      auto packs = [&](int V) {
+        return rw_packs(a.table, a.vocab, a.d, a.ld_table, sizeof(TI), V) &&
+               rw_packs(a.out, a.n, a.d, a.ld_out, sizeof(TO), V);
+      };
+      return packs(kV) ? embed_launch<TI, TO, kV>(a, s)
+             : packs(2) ? embed_launch<TI, TO, 2>(a, s) : embed_launch<TI, TO, 1>(a, s);
     });
   });
 }
@@ -879,7 +883,8 @@ GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
   g.pairs1 = take(n * 8);
   g.counts = take((uint64_t)g.parts * kRadix * 4);
   const uint64_t chunks =
-      std::max({chunk_plan(n, d, 1).chunks, chunk_plan(n, d, 4).chunks, chunk_plan(n, d, 8).chunks});
+      std::max({chunk_plan(n, d, 1).chunks, chunk_plan(n, d, 2).chunks, chunk_plan(n, d, 4).chunks,
+                chunk_plan(n, d, 8).chunks});
   g.partial = take(chunks * 2 * ((d + 3) / 4 * 4) * 4);
   // the table path keeps its CTAs' tables there instead
   if (table_fits(d, vocab))
@@ -950,7 +955,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   // Few ids, many rows: the whole table is zeroed beside the sort and the rows that ids name
   // are written again, instead of looking for each row among the ids (512 ids into 32000 x
   // 768: 30 -> 21 us).
-  const bool zero_first = count && !a.accumulate && a.n <= a.vocab / 8;
+  const bool zero_first = count && !a.accumulate && a.n <= a.vocab / 4;
   if (count) {
     *nl += 1;
     e = rw_with_index(a.id_type, [&](auto id) {
@@ -993,15 +998,19 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
       using TG = decltype(tg);
       using TD = decltype(td);
       constexpr int kV = 16 / sizeof(TG);
-      const bool wide = rw_packs(a.grad, a.n, a.d, a.ld_grad, sizeof(TG), kV) &&
-                        rw_packs(a.dtable, a.vocab, a.d, a.ld_dtable, sizeof(TD), kV);
-      cp = chunk_plan(a.n, a.d, wide ? kV : 1);
-      const uint64_t zero = a.accumulate || zero_first ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
+      auto packs = [&](int V) {
+        return rw_packs(a.grad, a.n, a.d, a.ld_grad, sizeof(TG), V) &&
+               rw_packs(a.dtable, a.vocab, a.d, a.ld_dtable, sizeof(TD), V);
+      };
+      const int V = packs(kV) ? kV : packs(2) ? 2 : 1;
+      cp = chunk_plan(a.n, a.d, V);
+      // about 128 KB a zeroing CTA, so that the last ones do not decide the time
+      cp.zero_rows = (uint32_t)std::min<uint64_t>(
+          kZeroRows, std::max<uint64_t>(4, (128u << 10) / (a.d * sizeof(TD))));
+      const uint64_t zero = a.accumulate || zero_first ? 0 : (a.vocab + cp.zero_rows - 1) / cp.zero_rows;
       const dim3 grid((uint32_t)(cp.sum_ctas + zero));
-      return wide ? rw_launch(k_embed_chunks<TG, TD, kV>, grid, dim3(kSumThreads), 0, s, true, a, cp,
-                              pairs, partial)
-                  : rw_launch(k_embed_chunks<TG, TD, 1>, grid, dim3(kSumThreads), 0, s, true, a, cp,
-                              pairs, partial);
+      auto* k = V == kV ? k_embed_chunks<TG, TD, kV> : V == 2 ? k_embed_chunks<TG, TD, 2> : k_embed_chunks<TG, TD, 1>;
+      return rw_launch(k, grid, dim3(kSumThreads), 0, s, true, a, cp, pairs, partial);
     });
   });
   if (e != cudaSuccess) return e;

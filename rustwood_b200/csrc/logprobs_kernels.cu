@@ -100,19 +100,24 @@ __device__ __forceinline__ RowEnd row_end(const Sums& a) {
 __device__ __forceinline__ float scaled_difference(float x, float base, float scale) {
   return (x * 0.5f - base * 0.5f) * scale * 2.0f;
 }
+// A row's target and its margin, two dependent loads: the target's is issued before the row's
+// loads and the margin's after them, so that neither is waited for at the row's end.
+__device__ __forceinline__ int64_t target_of(const LogprobsLaunch& a, uint64_t i) {
+  if (!a.logp) return -1;
+  return a.target_type == RW_I64 ? ((const int64_t*)a.targets)[i] : ((const int32_t*)a.targets)[i];
+}
 template <typename T>
-__device__ __forceinline__ void write_row(const LogprobsLaunch& a, uint64_t i, const Sums& r, const RowEnd& e) {
+__device__ __forceinline__ float margin_at(const LogprobsLaunch& a, uint64_t i, int64_t target, bool& in) {
+  in = target >= 0 && (uint64_t)target < a.classes;
+  return in ? rw_widen(((const T*)a.x)[i * a.ld_x + target]) : 0.0f;
+}
+__device__ __forceinline__ void write_row(const LogprobsLaunch& a, uint64_t i, const Sums& r, const RowEnd& e,
+                                          float target, bool in) {
   if (a.row_max) a.row_max[i] = r.m;
   if (a.log_sum) a.log_sum[i] = e.log_sum;
   if (a.lse) a.lse[i] = a.scale * r.m + e.log_sum;
   if (a.entropy) a.entropy[i] = r.m == -kInf ? 0.0f : e.log_sum - a.scale * __fdividef(r.t, r.s);
-  if (a.logp) {
-    const int64_t c = a.target_type == RW_I64 ? ((const int64_t*)a.targets)[i] : ((const int32_t*)a.targets)[i];
-    float v = 0.0f;
-    if (c >= 0 && (uint64_t)c < a.classes)
-      v = scaled_difference(rw_widen(((const T*)a.x)[i * a.ld_x + c]), e.base, a.scale) - e.log_sum;
-    a.logp[i] = v;
-  }
+  if (a.logp) a.logp[i] = in ? scaled_difference(target, e.base, a.scale) - e.log_sum : 0.0f;
 }
 __device__ __forceinline__ void write_top(const LogprobsLaunch& a, uint64_t i, uint32_t place, Key k, const RowEnd& e) {
   if (a.top_index) a.top_index[i * a.top_k + place] = index_of(k);
@@ -124,12 +129,13 @@ __device__ __forceinline__ void write_top(const LogprobsLaunch& a, uint64_t i, u
 // Few classes: L lanes a row, at most E margins a lane, all in registers.
 
 constexpr int kGroupThreads = 256;
-constexpr uint32_t kCountPlaces = 6;
+constexpr uint32_t kCountPlaces = 6, kReducePlaces = 8;
 constexpr int kGroupCand = 128;  // candidates for a row's top places that a warp keeps
 
 template <typename T, int L, int E>
-__global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a) {
-  __shared__ Key s_cand[L == 32 ? kGroupThreads / 32 : 1][L == 32 ? kGroupCand : 1];
+__global__ void __launch_bounds__(kGroupThreads, L < 32 ? 1 : E <= 8 ? 6 : E <= 16 ? 4 : 3) k_logprobs_few(LogprobsLaunch a) {
+  __shared__ __align__(16) uint32_t s_cand[L == 32 ? kGroupThreads / 32 : 1][L == 32 ? kGroupCand : 1];
+  __shared__ uint32_t s_cand_at[L == 32 ? kGroupThreads / 32 : 1][L == 32 ? kGroupCand : 1];
   const uint32_t lane = threadIdx.x % L, classes = (uint32_t)a.classes;
   const float c = a.scale * kLog2e;
   constexpr uint32_t kRows = kGroupThreads / L;  // rows of a CTA at a time
@@ -137,12 +143,17 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
     const uint64_t i = base + threadIdx.x / L;
     const bool real = i < a.n;
     const T* x = (const T*)a.x + (real ? i : a.n - 1) * a.ld_x;
+    // rows that share a warp leave no registers for it (24.6 -> 26.8 us at 1000000 x 7 f32)
+    int64_t target = L == 32 && real && lane == 0 ? target_of(a, i) : -1;
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const uint32_t j = lane + e * L;
       v[e] = j < classes ? rw_widen(x[j]) : -kInf;
     }
+    bool in_row = false;
+    float at_target = 0.0f;
+    if (L == 32) at_target = margin_at<T>(a, i, target, in_row);
     Sums r;
 #pragma unroll
     for (int e = 0; e < E; e++) r.m = max_nan(r.m, v[e]);
@@ -163,34 +174,50 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
       r.t += __shfl_xor_sync(0xffffffffu, r.t, o);
     }
     const RowEnd end = row_end(r);
-    if (real && lane == 0) write_row<T>(a, i, r, end);
+    if (real && lane == 0) {
+      if (L < 32) at_target = margin_at<T>(a, i, target_of(a, i), in_row);
+      write_row(a, i, r, end, at_target, in_row);
+    }
     if (a.top_k == 0) continue;
+    uint32_t order[E];  // 0: no margin, or one that has its place
+#pragma unroll
+    for (int e = 0; e < E; e++) order[e] = lane + e * L < classes ? order_of(v[e]) : 0;
     if constexpr (L == 32) {
       // The top_k-th largest of the lanes' maxima is a bound: top_k margins at least reach it.
       // Those that do (the bound's own included) are ranked by counting. Too many only if
       // many are equal or a lane holds many of the largest: then place by place, below.
-      const uint32_t mine = order_of(own);
-      uint32_t above = 0;
+      uint32_t left = order_of(own), bound = 0;
+      if (a.top_k <= kReducePlaces) {  // maximum by maximum
+        for (uint32_t found = 0;;) {
+          bound = __reduce_max_sync(0xffffffffu, left);
+          found += __popc(__ballot_sync(0xffffffffu, left == bound));
+          if (found >= a.top_k) break;
+          if (left == bound) left = 0;
+        }
+      } else {  // the largest that top_k lanes reach
+        uint32_t reach = 0;
 #pragma unroll
-      for (int o = 0; o < 32; o++) {
-        const uint32_t other = __shfl_sync(0xffffffffu, mine, o);
-        above += other > mine || (other == mine && o < (int)lane);
+        for (int o = 0; o < 32; o++) reach += __shfl_sync(0xffffffffu, left, o) >= left;
+        bound = __reduce_max_sync(0xffffffffu, reach >= a.top_k ? left : 0u);
       }
-      const uint32_t who = __ballot_sync(0xffffffffu, above == a.top_k - 1);
-      const uint32_t bound = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
-      Key* cand = s_cand[threadIdx.x / 32];
+      // the candidates' orders and indices, in index order
+      uint32_t* cand = s_cand[threadIdx.x / 32];
+      uint32_t* cand_at = s_cand_at[threadIdx.x / 32];
       auto collect = [&](uint32_t from) {
         uint32_t count = 0;
         __syncwarp();
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          const uint32_t o = order_of(v[e]);
-          const bool in = o >= from && lane + e * 32 < classes;
-          const uint32_t hits = __ballot_sync(0xffffffffu, in);
+          const uint32_t hits = __ballot_sync(0xffffffffu, order[e] >= from);
+          if (hits == 0) continue;
           const uint32_t at = count + __popc(hits & ((1u << lane) - 1));
-          if (in && at < kGroupCand) cand[at] = key_of(o, lane + e * 32);
+          if (order[e] >= from && at < kGroupCand) {
+            cand[at] = order[e];
+            cand_at[at] = lane + e * 32;
+          }
           count += __popc(hits);
         }
+        if (lane < 4 && count + lane < kGroupCand) cand[count + lane] = 0;
         __syncwarp();
         return count;
       };
@@ -202,17 +229,22 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
       }
       if (count <= kGroupCand) {
         for (uint32_t q = lane; q < count; q += 32) {
-          const Key k = cand[q];
+          // those above it, and the equal ones before it: whole fours by >=, then its own four
+          const uint32_t k = cand[q], four = q & ~3u;
           uint32_t place = 0;
-#pragma unroll 4
-          for (uint32_t w = 0; w < count; w++) place += cand[w] > k;
-          if (real && place < a.top_k) write_top(a, i, place, k, end);
+          for (uint32_t w = 0; w < count; w += 4) {
+            const uint4 o = *(const uint4*)(cand + w);
+            const uint32_t than = w < four ? k - 1 : k;  // orders are above 0
+            place += (o.x > than) + (o.y > than) + (o.z > than) + (o.w > than);
+          }
+          for (uint32_t w = four; w < q; w++) place += cand[w] == k;
+          if (real && place < a.top_k) write_top(a, i, place, key_of(k, cand_at[q]), end);
         }
         uint32_t place = a.top_k - ties;
 #pragma unroll
         for (int e = 0; e < E; e++) {
           if (place >= a.top_k) break;
-          const bool in = order_of(v[e]) == bound && lane + e * 32 < classes;
+          const bool in = order[e] == bound;
           const uint32_t hits = __ballot_sync(0xffffffffu, in);
           const uint32_t at = place + __popc(hits & ((1u << lane) - 1));
           if (real && in && at < a.top_k) write_top(a, i, at, key_of(bound, lane + e * 32), end);
@@ -221,11 +253,7 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
         continue;
       }
     }
-    // place by place; a margin that has its place has order 0 from then on
-    uint32_t order[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) order[e] = lane + e * L < classes ? order_of(v[e]) : 0;
-    if constexpr (L * E <= 32) {
+    if constexpr (L > 1 && L * E <= 32) {
       // many places of few margins: every margin counts those before it
       if (a.top_k > kCountPlaces) {
         uint32_t above[E];
@@ -250,6 +278,7 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
         continue;
       }
     }
+    // place by place
     for (uint32_t place = 0; place < a.top_k; place++) {
       uint32_t top = order[0], at = lane;
 #pragma unroll
@@ -277,7 +306,7 @@ __global__ void __launch_bounds__(kGroupThreads) k_logprobs_few(LogprobsLaunch a
 // Threads a CTA: 256, or 64 for many short rows, whose barriers and joins cost more than
 // their margins (48056 x 2824 bf16: 344 -> XX us).
 constexpr int kRowThreads = 256, kShortThreads = 64;
-constexpr uint64_t kShortBytes = 32 << 10;
+constexpr uint64_t kShortBytes = 64 << 10;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
 constexpr uint32_t kGroups = 64;   // groups of threads whose maxima bound the top places
 constexpr uint32_t kCand = 1024;   // candidates for the top places that a CTA keeps
@@ -385,7 +414,7 @@ struct TopSpace {
   // reach it, many margins equal it.
   static constexpr uint32_t kLook = kMaxTop * kGroupSize;
   uint32_t order[NT];  // each thread's largest
-  uint32_t group[kGroups];
+  alignas(16) uint32_t group[kGroups];
   Key cand[kCand];
   uint32_t warp[kWarps];
   Key warp_key[kWarps];
@@ -399,7 +428,7 @@ struct TopSpace {
 template <int NT>
 __device__ __forceinline__ void top_threads(float own, TopSpace<NT>& s) {
   s.order[threadIdx.x] = order_of(own);
-  if (threadIdx.x == 0) s.count = s.looking = 0;
+  if (threadIdx.x == 0) s.count = s.looking = s.bound = 0;
 }
 template <int NT>
 __device__ __forceinline__ void top_groups(TopSpace<NT>& s) {
@@ -421,19 +450,21 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   constexpr int kV = Span<T>::kV;
   const uint32_t mine = order_of(own);
-  // A bound that top_k margins at least reach: the top_k-th largest of the groups' maxima,
-  // found by counting; the kGroupSize threads of a group share the comparisons.
+  // A bound that top_k margins at least reach: the largest of the groups' maxima that top_k
+  // groups reach; the kGroupSize threads of a group share the comparisons.
   {
-    const uint32_t at = t / kGroupSize, g = s.group[at];
-    uint32_t above = 0;
+    constexpr uint32_t kEach = kGroups / kGroupSize;
+    const uint32_t g = s.group[t / kGroupSize], first = t % kGroupSize * kEach;
+    uint32_t reach = 0;
 #pragma unroll
-    for (uint32_t u = 0; u < kGroups / kGroupSize; u++) {
-      const uint32_t q = t % kGroupSize + u * kGroupSize, o = s.group[q];
-      above += o > g || (o == g && q < at);
+    for (uint32_t q = 0; q < kEach; q += 4) {
+      const uint4 o = *(const uint4*)(s.group + first + q);
+      reach += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
     }
 #pragma unroll
-    for (uint32_t o = kGroupSize / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-    if (above == top_k - 1) s.bound = g;  // one group's threads
+    for (uint32_t o = kGroupSize / 2; o > 0; o >>= 1) reach += __shfl_xor_sync(0xffffffffu, reach, o);
+    const uint32_t best = __reduce_max_sync(0xffffffffu, reach >= top_k ? g : 0u);
+    if (lane == 0) atomicMax(&s.bound, best);
   }
   __syncthreads();
   const uint32_t bound = s.bound;
@@ -585,6 +616,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
   const Span<T> sp((const T*)a.x + i * a.ld_x + lo, (uint32_t)(hi - lo));
   rw_let_successor_start();  // k_logprobs_join of a split row waits for this kernel
   const float c = a.scale * kLog2e;
+  const int64_t target = t == 0 && sr.parts == 1 ? target_of(a, i) : -1;
 
   float m = -kInf, mc = 0.0f;
   Two s = 0, w = 0, c2 = two_of(c, c), base = 0;  // base: -mc twice
@@ -652,6 +684,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
     p.load(sp.vec(v));
     absorb(&p, kOnePack);
   }
+  bool in_row;
+  const float at_target = margin_at<T>(a, i, target, in_row);
   Sums r;
   r.m = m;
   if (!(m <= kLowest)) {
@@ -687,7 +721,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
   r = {all, sums.x, sums.y};
   if (sr.parts == 1) {
     const RowEnd end = row_end(r);
-    if (t == 0) write_row<T>(a, i, r, end);
+    if (t == 0) write_row(a, i, r, end, at_target, in_row);
     if (a.top_k)
       top_places(sp, 0u, own, a.top_k, s_top, [&](uint32_t place, Key k) { write_top(a, i, place, k, end); });
   } else {
@@ -719,6 +753,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
   const float c = a.scale * kLog2e;
   rw_dependent_start();
   // everything that is read is on its way before anything is waited for
+  const int64_t target = t == kJoinThreads - 1 ? target_of(a, i) : -1;
   const Sums* sums = sr.sums + i * sr.parts;
   Sums r, r2;
   if (lane < sr.parts) r = sums[lane];
@@ -730,6 +765,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
     const uint32_t list = warp + u * (kJoinThreads / 32);
     held[u] = list < sr.parts && lane < a.top_k ? keys[list * a.top_k + lane] : 0;
   }
+  bool in_row;
+  const float at_target = margin_at<T>(a, i, target, in_row);
   if (t < sr.parts && a.top_k) s_head[t] = keys[(uint64_t)t * a.top_k];
   if (t == 0) {
     s_count = 0;
@@ -740,7 +777,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
   for (int o = 16; o > 0; o >>= 1) r = join(r, shuffle_xor(r, o), c);
   const RowEnd end = row_end(r);
   if (a.top_k == 0) {
-    if (t == 0) write_row<T>(a, i, r, end);
+    if (t == kJoinThreads - 1) write_row(a, i, r, end, at_target, in_row);
     return;
   }
   __syncthreads();
@@ -766,7 +803,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
     for (uint32_t w = 0; w < count; w++) place += s_cand[w] > k;
     if (place < a.top_k) write_top(a, i, place, k, end);
   }
-  if (t == kJoinThreads - 1) write_row<T>(a, i, r, end);  // the warp with the least to do above
+  if (t == kJoinThreads - 1) write_row(a, i, r, end, at_target, in_row);
 }
 
 // =================================================================================
@@ -933,8 +970,23 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGrad
     if (VEC && j0 + kV <= total) {
       Pack<T, kV> p;
       p.load(x + j0);
+      const uint32_t row = row_of(j0), j = j0 - row * classes;
+      const int32_t target = s_target[row];
+      if (kV > 1 && classes >= 16 * kV && !formula && j + kV <= classes && (uint32_t)(target - (int32_t)j) >= kV) {
+        // one row's, and the target elsewhere
+        const float4 r = s_row[row];
+        const Two c2 = two_of(c, c), k2 = two_of(-r.x, -r.x), a2 = two_of(-r.y, -r.y), b2 = two_of(-r.z, -r.z);
 #pragma unroll
-      for (int k = 0; k < kV; k++) p.set(k, element(j0 + k, row_of(j0 + k), p.get(k)));
+        for (int q = 0; q < kV / 2; q++) {
+          const Two d = fma2(pair_of<true>(p, q), c2, k2);
+          const float2 df = both(d), w = both(fma2(b2, d, a2));
+          p.set(2 * q, target == -2 ? 0.0f : exp2_fast(df.x) * w.x);
+          p.set(2 * q + 1, target == -2 ? 0.0f : exp2_fast(df.y) * w.y);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kV; k++) p.set(k, element(j0 + k, row_of(j0 + k), p.get(k)));
+      }
       p.store(dx + j0);
     } else {
       for (uint32_t at = j0; at < min(total, j0 + kV); at++) {
@@ -989,7 +1041,9 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
       if (a.classes <= 128)
         return a.top_k <= 4 ? go(k_logprobs_few<T, 8, 16>, 8) : go(k_logprobs_few<T, 32, 4>, 32);
       if (a.classes <= 256) return go(k_logprobs_few<T, 32, 8>, 32);
+      if (a.classes <= 384) return go(k_logprobs_few<T, 32, 12>, 32);
       if (a.classes <= 512) return go(k_logprobs_few<T, 32, 16>, 32);
+      if (a.classes <= 768) return go(k_logprobs_few<T, 32, 24>, 32);
       return go(k_logprobs_few<T, 32, 32>, 32);
     });
   SplitRow r = split_of(a.n, a.classes);
@@ -1013,8 +1067,9 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
   });
 }
 
-// Up to this many classes rows share CTAs.
-constexpr uint64_t kGradFew = 2048;
+// Up to this many classes whole rows share CTAs where they are one run of vectors (a CTA of
+// one row would have too little to do), else up to kGradFewStrided.
+constexpr uint64_t kGradFew = 8192, kGradFewStrided = 1024;
 
 cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, int* nl) {
   if (a.n == 0 || a.classes == 0) return cudaSuccess;
@@ -1025,8 +1080,9 @@ cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, in
     const dim3 block(kGradThreads);
     const uintptr_t x = (uintptr_t)a.x, dx = (uintptr_t)a.dx;
     const bool one = a.n == 1;
-    if (a.classes <= kGradFew) {
-      const bool vec = x % 16 == 0 && dx % 16 == 0 && (one || (a.ld_x == a.classes && a.ld_dx == a.classes));
+    const bool run = x % 16 == 0 && dx % 16 == 0 && (one || (a.ld_x == a.classes && a.ld_dx == a.classes));
+    if (a.classes <= (run ? kGradFew : kGradFewStrided)) {
+      const bool vec = run;
       // about kGradDepth vectors a thread, whole vectors in whole rows
       uint64_t rows = kGradThreads * kGradDepth * kV / a.classes;
       rows = std::min<uint64_t>(std::max<uint64_t>(rows, 1) + kV - 1, kGradRows) / kV * kV;

@@ -880,6 +880,7 @@ extern "C" int rw_embed_device(rw_ctx* ctx, const void* d_table, int32_t table_t
       [&]() -> std::string {
         if (!elem_type_ok(table_type) || !elem_type_ok(out_type)) return "unknown element type";
         if (!index_type_ok(id_type)) return "unknown id type";
+        if (d > kMaxWidth) return "d must be below 2^23";
         RW_MATRIX(d_table, vocab, d, ld_table, elem_bytes(table_type));
         RW_VECTOR(d_ids, n, index_bytes(id_type));
         RW_MATRIX(d_out, n, d, ld_out, elem_bytes(out_type));

@@ -52,6 +52,7 @@ CASES = [
     (embed, dict(table_type=3), "unknown element type"),
     (embed, dict(out_type=-1), "unknown element type"),
     (embed, dict(id_type=2), "unknown id type"),
+    (embed, dict(d=1 << 23, ld_table=1 << 23, ld_out=1 << 23), "below 2^23"),
     (embed, dict(table=None), "d_table is NULL"),
     (embed, dict(ids=None), "d_ids is NULL"),
     (embed, dict(out=None), "d_out is NULL"),
