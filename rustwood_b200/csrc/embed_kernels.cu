@@ -299,7 +299,8 @@ __device__ __forceinline__ uint64_t lower_bound(const unsigned long long* pairs,
 template <typename TG, typename TD, int V>
 __global__ void __launch_bounds__(kSumThreads)
     k_embed_chunks(EmbedGradLaunch a, ChunkPlan cp, const unsigned long long* __restrict__ pairs,
-                   float* __restrict__ partial) {
+                   float* __restrict__ partial, uint2* __restrict__ ends) {
+  constexpr int kDepth = kSumDepth;
   const uint32_t slot = threadIdx.x / cp.tx, lane = threadIdx.x % cp.tx;
   TD* dtable = (TD*)a.dtable;
   rw_dependent_start();
@@ -353,16 +354,22 @@ __global__ void __launch_bounds__(kSumThreads)
     }
   };
 
-  for (uint64_t j = lo; j < hi; j += kSumDepth) {
-    unsigned long long pair[kSumDepth];
-    Pack<TG, V> row[kSumDepth];
+  // the next round's pairs are on their way while this round's rows are
+  unsigned long long next[kDepth];
 #pragma unroll
-    for (int u = 0; u < kSumDepth; u++) pair[u] = j + u < hi ? pairs[j + u] : ~0ull;
+  for (int u = 0; u < kDepth; u++) next[u] = lo + u < hi ? pairs[lo + u] : ~0ull;
+  for (uint64_t j = lo; j < hi; j += kDepth) {
+    unsigned long long pair[kDepth];
+    Pack<TG, V> row[kDepth];
 #pragma unroll
-    for (int u = 0; u < kSumDepth; u++)
+    for (int u = 0; u < kDepth; u++) pair[u] = next[u];
+#pragma unroll
+    for (int u = 0; u < kDepth; u++)
       if (key_of(pair[u]) < a.vocab) row[u].load(grad + (uint64_t)(uint32_t)pair[u] * a.ld_grad);
 #pragma unroll
-    for (int u = 0; u < kSumDepth; u++) {
+    for (int u = 0; u < kDepth; u++) next[u] = j + kDepth + u < hi ? pairs[j + kDepth + u] : ~0ull;
+#pragma unroll
+    for (int u = 0; u < kDepth; u++) {
       if (j + u >= hi) break;
       const uint32_t key = key_of(pair[u]);
       if (key != run) {
@@ -379,6 +386,7 @@ __global__ void __launch_bounds__(kSumThreads)
     }
   }
   flush(hi < a.n && key_of(pairs[hi]) == run);
+  if (col == 0) ends[chunk] = make_uint2(key_of(pairs[lo]), key_of(pairs[hi - 1]));
 }
 
 // Adds the partial sums of the runs that cross chunks: CTA (x, y) takes the runs that start
@@ -387,12 +395,12 @@ __global__ void __launch_bounds__(kSumThreads)
 // has fewer than 32 float4s, groups of lanes take every 2nd, 4th, .. chunk.
 template <typename TD>
 __global__ void __launch_bounds__(kJoinThreads)
-    k_embed_join(EmbedGradLaunch a, ChunkPlan cp, const unsigned long long* __restrict__ pairs,
-                 const float* __restrict__ partial) {
+    k_embed_join(EmbedGradLaunch a, ChunkPlan cp, const float* __restrict__ partial,
+                 const uint2* __restrict__ ends) {  // a chunk's first and last id
   constexpr int kWarps = kJoinThreads / 32;
   constexpr uint32_t kLong = 24;  // chunks from which on a run is shared by the warps
-  __shared__ uint32_t s_first[kJoinThreads], s_last[kJoinThreads];
-  __shared__ uint32_t s_count;
+  __shared__ uint32_t s_first[kJoinThreads], s_shared[kJoinThreads];  // runs; those all warps share
+  __shared__ uint32_t s_count, s_long;
   __shared__ float4 s_part[kWarps][32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t width = cp.join_lanes, groups = 32 / width, group = lane / width;
@@ -423,8 +431,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   };
   auto finish = [&](uint32_t first, float4 s) {
     if (group != 0) return;
-    const uint64_t end = min((uint64_t)(first + 1) * cp.chunk, a.n);
-    TD* p = dtable + (uint64_t)key_of(pairs[end - 1]) * a.ld_dtable + col;
+    TD* p = dtable + (uint64_t)ends[first].y * a.ld_dtable + col;
     const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -433,40 +440,42 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
   };
 
+  // The last chunk of the run that starts in chunk `first`, by a warp: 32 probes at a time, at
+  // doubling distances and then evenly spaced.
+  auto last_of = [&](uint32_t first) {
+    const uint32_t key = ends[first].y;
+    auto probe = [&](uint64_t q) {  // the number of lanes whose chunk begins with the run's id
+      return (uint32_t)__popc(__ballot_sync(0xffffffffu, q < cp.chunks && ends[q].x == key));
+    };
+    uint32_t step = 1u << (probe((uint64_t)first + (1u << min(lane, 20u))) - 1);  // chunk first + 1 does
+    uint64_t last = (uint64_t)first + step;
+    while (step > 1) {  // the end is less than `step` chunks on
+      step = (step + 31) / 32;
+      last += (uint64_t)step * probe(last + (uint64_t)step * (lane + 1));
+    }
+    return (uint32_t)last;
+  };
+
   for (uint64_t base = 0; base < cp.chunks; base += (uint64_t)gridDim.x * kJoinThreads) {
     __syncthreads();
-    if (threadIdx.x == 0) s_count = 0;
+    if (threadIdx.x == 0) s_count = s_long = 0;
     __syncthreads();
     const uint64_t c = base + blockIdx.x + (uint64_t)threadIdx.x * gridDim.x;
     if (c + 1 < cp.chunks) {
-      const uint64_t lo = c * cp.chunk, hi = lo + cp.chunk;
-      const uint32_t key = key_of(pairs[hi - 1]);
-      if (key < a.vocab && key_of(pairs[hi]) == key && (lo == 0 || key_of(pairs[lo - 1]) != key)) {
-        // the last chunk that begins with this id: in growing steps, then by halving
-        uint64_t in = c + 1, out = cp.chunks;
-        for (uint64_t step = 1; in + step < out; step *= 2) {
-          if (key_of(pairs[(in + step) * cp.chunk]) == key) in += step;
-          else out = in + step;
-        }
-        while (out - in > 1) {
-          const uint64_t mid = (in + out) / 2;
-          if (key_of(pairs[mid * cp.chunk]) == key) in = mid;
-          else out = mid;
-        }
-        const uint32_t at = atomicAdd(&s_count, 1u);  // the list's order does not matter
-        s_first[at] = (uint32_t)c;
-        s_last[at] = (uint32_t)in;
-      }
+      const uint32_t key = ends[c].y;
+      if (key < a.vocab && ends[c + 1].x == key && (c == 0 || ends[c - 1].y != key))
+        s_first[atomicAdd(&s_count, 1u)] = (uint32_t)c;  // the list's order does not matter
     }
     __syncthreads();
     const uint32_t count = s_count;
     for (uint32_t k = warp; k < count; k += kWarps) {
-      const uint32_t first = s_first[k], last = s_last[k];
+      const uint32_t first = s_first[k], last = last_of(first);
       if (last - first < kLong) finish(first, row_sum(first, first, last + 1));
+      else if (lane == 0) s_shared[atomicAdd(&s_long, 1u)] = first;
     }
-    for (uint32_t k = 0; k < count; k++) {
-      const uint32_t first = s_first[k], last = s_last[k];
-      if (last - first < kLong) continue;
+    __syncthreads();
+    for (uint32_t k = 0; k < s_long; k++) {
+      const uint32_t first = s_shared[k], last = last_of(first);
       const uint32_t m = last + 1 - first, per = (m + kWarps - 1) / kWarps;
       const uint32_t lo = min(m, warp * per), hi = min(m, lo + per);
       s_part[warp][lane] = row_sum(first, first + lo, first + hi);
@@ -778,7 +787,9 @@ cudaError_t embed_launch(const EmbedLaunch& a, cudaStream_t s) {
   // row where a row has four warps' worth, else of two or four rows
   const bool many = a.n >= 8 * kSms;
   const uint32_t warps = (ep.dv + 31) / 32;
-  const int c = !many ? 1 : warps >= 4 ? 4 : warps >= 2 ? 2 : 1, r = many ? 4 / c : 1;
+  int c = !many ? 1 : warps >= 4 ? 4 : warps >= 2 ? 2 : 1;
+  const int r = many ? 4 / c : 1;
+  if (V <= 2 && c == 4 && warps >= 8) c = 8;  // narrow loads: more of them
   uint64_t tx = ep.dv;
   if (c > 1) tx = ((ep.dv + c - 1) / c + 31) / 32 * 32;
   ep.tx = (uint32_t)std::min<uint64_t>(tx, kEmbedThreads);
@@ -788,6 +799,8 @@ cudaError_t embed_launch(const EmbedLaunch& a, cudaStream_t s) {
   ep.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 2 * kSms / groups));
   if (groups * ep.split > 0x7fffffffull) return cudaErrorInvalidValue;
   const dim3 grid((uint32_t)(groups * ep.split)), block(kEmbedThreads);
+  if constexpr (V <= 2)
+    if (c == 8) return rw_launch(k_embed<TI, TO, V, 1, 8>, grid, block, 0, s, false, a, ep);
   if (c == 4) return rw_launch(k_embed<TI, TO, V, 1, 4>, grid, block, 0, s, false, a, ep);
   if (c == 2) return rw_launch(k_embed<TI, TO, V, 2, 2>, grid, block, 0, s, false, a, ep);
   return many ? rw_launch(k_embed<TI, TO, V, 4, 1>, grid, block, 0, s, false, a, ep)
@@ -821,7 +834,7 @@ namespace {
 struct GradPlan {
   uint64_t part;
   uint32_t parts, passes;
-  uint64_t pairs0, pairs1, counts, partial, bytes;  // offsets
+  uint64_t pairs0, pairs1, counts, partial, ends, bytes;  // offsets
 };
 
 // Chunks: enough for about 16 CTAs an SM where a row takes two warps or more, so that the
@@ -886,6 +899,7 @@ GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
       std::max({chunk_plan(n, d, 1).chunks, chunk_plan(n, d, 2).chunks, chunk_plan(n, d, 4).chunks,
                 chunk_plan(n, d, 8).chunks});
   g.partial = take(chunks * 2 * ((d + 3) / 4 * 4) * 4);
+  g.ends = take(chunks * sizeof(uint2));
   // the table path keeps its CTAs' tables there instead
   if (table_fits(d, vocab))
     for (size_t elem : {2, 4})
@@ -991,6 +1005,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   if (e != cudaSuccess) return e;
   const unsigned long long* pairs = count ? buf[0] : buf[(g.passes + 1) & 1];
   float* partial = (float*)(ws + g.partial);
+  uint2* ends = (uint2*)(ws + g.ends);
   *nl += 2;
   ChunkPlan cp = {};
   e = rw_with_type(a.grad_type, [&](auto tg) {
@@ -1004,13 +1019,14 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
       };
       const int V = packs(kV) ? kV : packs(2) ? 2 : 1;
       cp = chunk_plan(a.n, a.d, V);
-      // about 128 KB a zeroing CTA, so that the last ones do not decide the time
+      // A zeroing CTA takes 128 KB, so that its search among the ids is a small part of it, or
+      // more where that still leaves 32 an SM, so that the last ones do not decide the time.
       cp.zero_rows = (uint32_t)std::min<uint64_t>(
-          kZeroRows, std::max<uint64_t>(4, (128u << 10) / (a.d * sizeof(TD))));
+          kZeroRows, std::max<uint64_t>({4, a.vocab / (kSms * 32), (128u << 10) / (a.d * sizeof(TD))}));
       const uint64_t zero = a.accumulate || zero_first ? 0 : (a.vocab + cp.zero_rows - 1) / cp.zero_rows;
       const dim3 grid((uint32_t)(cp.sum_ctas + zero));
       auto* k = V == kV ? k_embed_chunks<TG, TD, kV> : V == 2 ? k_embed_chunks<TG, TD, 2> : k_embed_chunks<TG, TD, 1>;
-      return rw_launch(k, grid, dim3(kSumThreads), 0, s, true, a, cp, pairs, partial);
+      return rw_launch(k, grid, dim3(kSumThreads), 0, s, true, a, cp, pairs, partial, ends);
     });
   });
   if (e != cudaSuccess) return e;
@@ -1018,7 +1034,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   const uint32_t gx = std::max(1u, std::min(cp.chunks, (uint32_t)kSms * 4 / cols));
   return rw_with_type(a.dtable_type, [&](auto td) {
     return rw_launch(k_embed_join<decltype(td)>, dim3(gx, cols), dim3(kJoinThreads), 0, s, true, a,
-                     cp, pairs, (const float*)partial);
+                     cp, (const float*)partial, (const uint2*)ends);
   });
 }
 
