@@ -5,8 +5,8 @@
 //   gradient  dtable[v] (+)= scale * sum over i with ids[i] = v of grad[i]
 //   dropout   y[e] = keep(e) ? x[e] / (1 - p) : 0
 //
-// All three move bytes: nothing is computed that the memory does not bound. An id outside
-// the table is padding: a zero row, and no gradient.
+// All three are bound by the bytes they move. An id outside the table is padding: a zero row,
+// and no gradient.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -24,7 +24,8 @@ constexpr int kSms = 148;
 
 // `tx` threads a row, V columns a thread and access; a thread takes R rows and C vectors of
 // each at a time, all in flight, so that short rows have as much in flight as long ones. Every
-// CTA takes slots * R rows and is done.
+// CTA takes slots * R rows and is done. 65536 x 4096 bf16: 131 us, 5.3 TB/s of the bytes that
+// have to move; 136 us with a resident grid, 167 us with two vectors in flight.
 constexpr int kEmbedThreads = 256;
 
 struct EmbedPlan {
@@ -82,7 +83,8 @@ __global__ void __launch_bounds__(kEmbedThreads) k_embed(EmbedLaunch a, EmbedPla
 //
 // The sort is a radix sort over (id, position) pairs, digits of at most 9 bits, two
 // launches a pass: digit counts per part of the input, then a stable scatter in which
-// every CTA derives its part's bases from the counts of all parts.
+// every CTA derives its part's bases from the counts of all parts. 65536 ids of 128000: two
+// passes, 22 us of chained latencies for 2 MB.
 
 constexpr int kRadixBits = 9;
 constexpr int kRadix = 1 << kRadixBits;
@@ -262,14 +264,15 @@ __global__ void __launch_bounds__(kCountThreads)
 // A run of equal ids inside one chunk is finished there; a run that crosses chunks leaves
 // an f32 partial sum in each of them, and k_embed_join adds those in the chunks' order. So
 // a frequent id is summed by many slots, and the order of every addition is fixed by the
-// ids and the sizes.
+// ids and the sizes. Rows that no id names are zeroed by further CTAs of the same launch.
+// 65536 x 4096 bf16 into 128000 rows f32: 441 us for 2.6 GB, 6.0 TB/s; 482 us with the sort
+// and the join.
 
 constexpr int kSumThreads = 256;
 constexpr int kSumDepth = 4;    // rows in flight per thread
 constexpr int kZeroRows = 128;  // the most table rows a zeroing CTA covers
 constexpr int kJoinThreads = 512;
 constexpr int kJoinCols = 128;  // columns of one join (a float4 a lane)
-constexpr uint32_t kNone = 0xffffffffu;
 
 struct ChunkPlan {
   uint32_t chunk;       // positions a chunk
@@ -300,7 +303,6 @@ template <typename TG, typename TD, int V>
 __global__ void __launch_bounds__(kSumThreads)
     k_embed_chunks(EmbedGradLaunch a, ChunkPlan cp, const unsigned long long* __restrict__ pairs,
                    float* __restrict__ partial, uint2* __restrict__ ends) {
-  constexpr int kDepth = kSumDepth;
   const uint32_t slot = threadIdx.x / cp.tx, lane = threadIdx.x % cp.tx;
   TD* dtable = (TD*)a.dtable;
   rw_dependent_start();
@@ -355,21 +357,21 @@ __global__ void __launch_bounds__(kSumThreads)
   };
 
   // the next round's pairs are on their way while this round's rows are
-  unsigned long long next[kDepth];
+  unsigned long long next[kSumDepth];
 #pragma unroll
-  for (int u = 0; u < kDepth; u++) next[u] = lo + u < hi ? pairs[lo + u] : ~0ull;
-  for (uint64_t j = lo; j < hi; j += kDepth) {
-    unsigned long long pair[kDepth];
-    Pack<TG, V> row[kDepth];
+  for (int u = 0; u < kSumDepth; u++) next[u] = lo + u < hi ? pairs[lo + u] : ~0ull;
+  for (uint64_t j = lo; j < hi; j += kSumDepth) {
+    unsigned long long pair[kSumDepth];
+    Pack<TG, V> row[kSumDepth];
 #pragma unroll
-    for (int u = 0; u < kDepth; u++) pair[u] = next[u];
+    for (int u = 0; u < kSumDepth; u++) pair[u] = next[u];
 #pragma unroll
-    for (int u = 0; u < kDepth; u++)
+    for (int u = 0; u < kSumDepth; u++)
       if (key_of(pair[u]) < a.vocab) row[u].load(grad + (uint64_t)(uint32_t)pair[u] * a.ld_grad);
 #pragma unroll
-    for (int u = 0; u < kDepth; u++) next[u] = j + kDepth + u < hi ? pairs[j + kDepth + u] : ~0ull;
+    for (int u = 0; u < kSumDepth; u++) next[u] = j + kSumDepth + u < hi ? pairs[j + kSumDepth + u] : ~0ull;
 #pragma unroll
-    for (int u = 0; u < kDepth; u++) {
+    for (int u = 0; u < kSumDepth; u++) {
       if (j + u >= hi) break;
       const uint32_t key = key_of(pair[u]);
       if (key != run) {
@@ -717,8 +719,8 @@ constexpr int kDropoutDepth = 8 / (int)sizeof(T);  // 64 bytes
 // One thread takes the 8 elements of a counter, kDropoutDepth counters whose loads are all in
 // flight before it computes, and is done: many short CTAs overlap better than a resident grid
 // that walks the matrix with as many loads in flight (268M bf16: 185 us, 5.8 TB/s, against
-// 209-221 us). VEC: the matrices are contiguous and 16-byte aligned, so a
-// group is one or two 16-byte accesses; the last, partial one goes element by element.
+// 209-221 us). VEC: the matrices are contiguous and 16-byte aligned, so a group is one or two
+// 16-byte accesses; the last, partial one goes element by element.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256, kDropoutCtas) k_dropout(DropoutLaunch a, PhiloxKeys keys) {
   const uint64_t total = a.rows * a.cols;
@@ -774,10 +776,6 @@ __global__ void __launch_bounds__(256, kDropoutCtas) k_dropout(DropoutLaunch a, 
 uint32_t grid_of(uint64_t blocks, uint32_t per_sm) {
   return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(blocks, (uint64_t)kSms * per_sm));
 }
-
-}  // namespace
-
-namespace {
 
 template <typename TI, typename TO, int V>
 cudaError_t embed_launch(const EmbedLaunch& a, cudaStream_t s) {
@@ -909,10 +907,6 @@ GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
   return g;
 }
 
-}  // namespace
-
-namespace {
-
 ZeroRows zero_rows(void* p, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t elem) {
   const uint64_t pitch = ld * elem;
   ZeroRows z = {(char*)p, rows, 0, pitch, (uint32_t)elem};
@@ -1006,7 +1000,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
   const unsigned long long* pairs = count ? buf[0] : buf[(g.passes + 1) & 1];
   float* partial = (float*)(ws + g.partial);
   uint2* ends = (uint2*)(ws + g.ends);
-  *nl += 2;
+  *nl += 1;
   ChunkPlan cp = {};
   e = rw_with_type(a.grad_type, [&](auto tg) {
     return rw_with_type(a.dtable_type, [&](auto td) {
@@ -1029,7 +1023,8 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
       return rw_launch(k, grid, dim3(kSumThreads), 0, s, true, a, cp, pairs, partial, ends);
     });
   });
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || cp.chunks == 1) return e;
+  *nl += 1;
   const uint32_t cols = (uint32_t)((a.d + kJoinCols - 1) / kJoinCols);
   const uint32_t gx = std::max(1u, std::min(cp.chunks, (uint32_t)kSms * 4 / cols));
   return rw_with_type(a.dtable_type, [&](auto td) {

@@ -129,7 +129,17 @@ __device__ __forceinline__ void write_top(const LogprobsLaunch& a, uint64_t i, u
 // Few classes: L lanes a row, at most E margins a lane, all in registers.
 
 constexpr int kGroupThreads = 256;
-constexpr uint32_t kCountPlaces = 6, kReducePlaces = 8;
+// The places of at most 32 margins: one after another, or from more than kCountPlaces on by
+// counting (431527 x 15 f32, top 15: 112 us and 68 us).
+constexpr uint32_t kCountPlaces = 6;
+// The bound of a warp's row: by warp reductions, one a place, or above kReducePlaces by counting
+// (200000 x 100 bf16, top 5: 110 us and 123 us; top 10: 125 us and 128 us; top 20: 163 us and
+// 143 us).
+constexpr uint32_t kReducePlaces = 12;
+// Up to 128 classes: four rows a warp, or with more than kSharedPlaces places a warp a row
+// (200000 x 100 bf16, top 5: 80 us and 110 us; top 10: 132 us and 128 us; top 20: 235 us and
+// 143 us).
+constexpr uint32_t kSharedPlaces = 8;
 constexpr int kGroupCand = 128;  // candidates for a row's top places that a warp keeps
 
 template <typename T, int L, int E>
@@ -303,8 +313,9 @@ __global__ void __launch_bounds__(kGroupThreads, L < 32 ? 1 : E <= 8 ? 6 : E <= 
 // =================================================================================
 // Many classes: a CTA a row, or a part of one.
 
-// Threads a CTA: 256, or 64 for many short rows, whose barriers and joins cost more than
-// their margins (48056 x 2824 bf16: 344 -> XX us).
+// Threads a CTA: 256, or for many rows of at most kShortBytes 64, since barriers and joins cost
+// more than the margins of short rows (64 and 256 threads: 48056 x 2824 bf16 128 us and 344 us,
+// 8000 x 32000 115 us and 125 us; 6000 x 50000 136 us and 118 us).
 constexpr int kRowThreads = 256, kShortThreads = 64;
 constexpr uint64_t kShortBytes = 64 << 10;
 constexpr int kRowDepth = 4;       // vectors in flight a thread
@@ -589,7 +600,9 @@ __device__ __forceinline__ float2 cta_sum(float2 v, float2 (&s_tmp)[W]) {
   return v;
 }
 
-// One pass over a row (or part): 16-byte vectors, kRowDepth in flight, exponents as one
+// One pass over a row (or part): 16-byte vectors, kRowDepth in flight beside the kRowDepth that
+// are being summed (4096 x 128000 bf16 with entropy and top 5: 204 us, 5.1 TB/s; 337 us without
+// the second buffer), exponents as one
 // fused multiply-add e = x * c - mc with mc = round(m * c); the rounding of mc is known
 // exactly and taken out of the sums at the end. A thread restates its sums only when a block
 // of kRowDepth vectors holds a new maximum.
@@ -871,7 +884,8 @@ __device__ __forceinline__ float grad_element(const LogprobsGradLaunch& a, uint6
 }
 
 // Many classes: a CTA takes kGradThreads * kGradDepth vectors of one row. x and dx lie the
-// same distance from a 16-byte boundary (VEC), else it goes element by element.
+// same distance from a 16-byte boundary (VEC), else it goes element by element. 4096 x 128000
+// bf16 with entropy: 383 us, 5.5 TB/s, bound by the memory's mixed reads and writes.
 template <typename T, bool VEC, bool ENT>
 __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaunch a, uint32_t chunks) {
   constexpr int kV = Span<T>::kV;
@@ -926,7 +940,7 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaun
 
 // Few classes: a CTA takes `rows` whole rows, their constants in shared memory. VEC: the
 // matrices are contiguous and aligned, so the rows are one run of 16-byte vectors whose
-// elements may lie in different rows. magic = ceil(2^32 / classes): an element's row is the
+// elements may lie in different rows; 1000000 x 7 f32: 16 us, 4.2 TB/s. magic = ceil(2^32 / classes): an element's row is the
 // high half of its index times magic, exactly, as index * classes < 2^32.
 constexpr uint32_t kGradRows = 1024;
 
@@ -1002,6 +1016,7 @@ uint32_t grid_of(uint64_t blocks, uint32_t per_sm) {
   return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(blocks, 148ull * per_sm));
 }
 
+// Rows in registers up to here, by CTAs above (20000 x 1000 bf16, top 5: 36 us and 47 us).
 constexpr uint64_t kFewClasses = 1024;
 
 // Parts a row: with fewer rows than four CTAs an SM, enough parts to make that many, of 4096
@@ -1037,9 +1052,8 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
       };
       if (a.classes <= 8) return go(k_logprobs_few<T, 1, 8>, 1);
       if (a.classes <= 32) return go(k_logprobs_few<T, 4, 8>, 4);
-      // four rows a warp; many places are found faster with a warp a row
       if (a.classes <= 128)
-        return a.top_k <= 4 ? go(k_logprobs_few<T, 8, 16>, 8) : go(k_logprobs_few<T, 32, 4>, 32);
+        return a.top_k <= kSharedPlaces ? go(k_logprobs_few<T, 8, 16>, 8) : go(k_logprobs_few<T, 32, 4>, 32);
       if (a.classes <= 256) return go(k_logprobs_few<T, 32, 8>, 32);
       if (a.classes <= 384) return go(k_logprobs_few<T, 32, 12>, 32);
       if (a.classes <= 512) return go(k_logprobs_few<T, 32, 16>, 32);
@@ -1067,8 +1081,9 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
   });
 }
 
-// Up to this many classes whole rows share CTAs where they are one run of vectors (a CTA of
-// one row would have too little to do), else up to kGradFewStrided.
+// Up to this many classes whole rows share CTAs where they are one run of vectors, since a CTA
+// of one row would have too little to do (50000 x 2050 bf16: 96 us and 171 us), else up to
+// kGradFewStrided.
 constexpr uint64_t kGradFew = 8192, kGradFewStrided = 1024;
 
 cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, int* nl) {
