@@ -12,7 +12,8 @@
  *  - The caller owns every host buffer; outputs are written in full before return;
  *    no caller pointer is retained after a call returns.
  *  - A context (and the datasets/models created from it) is used by one host thread
- *    at a time. All device work of a context runs on one CUDA stream it owns.
+ *    at a time. All device work of a context runs on one CUDA stream it owns; only the
+ *    token operators run on the stream that the caller gives.
  *  - Model semantics are rustwood's: for tree t and level d, slot k = t*depth + d holds
  *    feat[k] (feature index) and thr[k] (raw cut value); a row's leaf index is built
  *    MSB-first as leaf = 2*leaf + (x[feat[k]] > thr[k]) (src/gpu_kernels.rs:1009),

@@ -20,6 +20,13 @@ pub const RW_OK: c_int = 0;
 pub const RW_OBJ_LOGISTIC: i32 = 0;
 pub const RW_OBJ_L2: i32 = 1;
 pub const RW_N_CATEGORIES: usize = 7;
+/// Element types and id types of the token operators, and the most alternatives per row.
+pub const RW_F32: i32 = 0;
+pub const RW_BF16: i32 = 1;
+pub const RW_F16: i32 = 2;
+pub const RW_I32: i32 = 0;
+pub const RW_I64: i32 = 1;
+pub const RW_MAX_TOP: u32 = 32;
 
 #[repr(C)]
 pub struct rw_ctx {
