@@ -302,7 +302,8 @@ int rw_target_transform(rw_ctx* ctx, float* x_rowmajor, uint64_t n, uint32_t nf,
  *    rw_*_workspace call gives, 256-byte aligned, with any contents; it must not be used
  *    by anything else until the stream has run the call. Calls that may run at the same
  *    time (two streams, two graphs) need a workspace each.
- *  - Results do not depend on timing: the same inputs give the same bits. */
+ *  - Results do not depend on timing: the same inputs, laid out the same, give the same
+ *    bits. */
 
 /* Element types (f32, bf16, f16) and the types of ids, targets and categories. */
 enum { RW_F32 = 0, RW_BF16 = 1, RW_F16 = 2 };
@@ -318,8 +319,8 @@ int rw_embed_device(rw_ctx* ctx, const void* d_table, int32_t table_type, uint64
 
 /* Its gradient: dtable[v] = scale * (the sum of grad[i] over i with ids[i] == v), zero for
  * rows no id names; with accumulate != 0 the sums are added to the rows that ids name and
- * the other rows are left as they were. Sums are f32 in an order that depends on ids alone,
- * rounded once to dtable_type. Ids outside 0..vocab-1 have no gradient. n, vocab < 2^31,
+ * the other rows are left as they were. Sums are f32 in an order that ids, sizes, strides
+ * and alignment fix, rounded once to dtable_type. Ids outside 0..vocab-1 have no gradient. n, vocab < 2^31,
  * d < 2^23. */
 int rw_embed_grad_workspace(rw_ctx* ctx, uint64_t n, uint64_t d, uint64_t vocab, uint64_t* bytes);
 int rw_embed_grad_device(rw_ctx* ctx, const void* d_grad, int32_t grad_type, uint64_t ld_grad,

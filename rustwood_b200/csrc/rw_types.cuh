@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+
 #include "rw_internal.cuh"
 
 __device__ __forceinline__ float rw_widen(float v) { return v; }
@@ -140,6 +142,15 @@ __device__ __forceinline__ void rw_dependent_start() {
 template <typename... KArgs, typename... Args>
 inline cudaError_t rw_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
                              bool dependent, Args... args) {
+  if (!dependent) {
+    std::tuple<std::remove_const_t<KArgs>...> held(args...);
+    return std::apply(
+        [&](auto&... a) {
+          void* at[] = {&a...};
+          return cudaLaunchKernel((const void*)k, grid, block, at, smem, s);
+        },
+        held);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -149,6 +160,6 @@ inline cudaError_t rw_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t 
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k, KArgs(args)...);
 }

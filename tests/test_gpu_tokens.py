@@ -193,13 +193,27 @@ def test_embed_and_its_gradient_are_adjoint(ctx):
     assert abs((up - left) - want) <= tol
 
 
+def test_lookup_and_its_gradient_past_32_bit_offsets(ctx):
+    """2^31 elements lie before the last rows of the output, and of the gradient that is summed."""
+    n, d = 530000, 4096
+    table = rand(1, 20, d, dtype=BF16)
+    ids = torch.arange(n, device="cuda") % 20
+    x = tokens.embed(ctx, table, ids)
+    assert torch.equal(x[-20:], table[ids[-20:]]) and torch.equal(x[:20], table)
+    x.zero_()
+    x[-40:] = rand(2, 40, d, dtype=BF16)
+    got = tokens.embed_grad(ctx, x, ids, 25)
+    check_grad(got, x[-40:], ids[-40:], 25, 1.0)
+
+
 # ---- dropout -----------------------------------------------------------------------------
 
 
-def philox_keep(n, p, seed, sequence):
-    """The kept elements, in numpy 64-bit integers (Philox4x32-10)."""
+def philox_keep(n, p, seed, sequence, first=0):
+    """Which of n elements from `first` (a multiple of 8) on are kept, in numpy 64-bit integers
+    (Philox4x32-10)."""
     m32 = np.uint64(0xFFFFFFFF)
-    g = np.arange((n + 7) // 8, dtype=np.uint64)
+    g = np.arange((n + 7) // 8, dtype=np.uint64) + np.uint64(first // 8)
     c = [g & m32, g >> np.uint64(32), np.full_like(g, sequence & 0xFFFFFFFF), np.full_like(g, sequence >> 32)]
     k0, k1 = seed & 0xFFFFFFFF, seed >> 32
     for _ in range(10):
@@ -245,6 +259,20 @@ def test_dropout(ctx, rows, cols, dtype):
         assert tokens.dropout(ctx, y, p, seed, seq, out=y) is y and torch.equal(y, want)
         offset = torch.cat([x.reshape(-1)[:1], x.reshape(-1)])[1:]  # one element off alignment
         assert torch.equal(tokens.dropout(ctx, offset, p, seed, seq), want.reshape(-1))
+
+
+@pytest.mark.parametrize("extra", [0, 3])
+def test_dropout_past_32_bit_offsets(ctx, extra):
+    """Elements around and beyond 2^31, contiguous and with rows further apart."""
+    rows, cols = 530000, 4096
+    buf = torch.ones(rows, cols + extra, device="cuda", dtype=BF16)
+    x = buf[:, :cols]
+    tokens.dropout(ctx, x, 0.25, 5, 6, out=x)
+    for row in (0, 524288, rows - 2):
+        keep = philox_keep(2 * cols, 0.25, 5, 6, first=row * cols)
+        want = torch.from_numpy(keep).cuda().reshape(2, cols) * torch.tensor(4 / 3, device="cuda")
+        assert torch.equal(x[row:row + 2], want.to(BF16))
+    assert (buf[:, cols:] == 1).all()
 
 
 def test_dropout_ends_of_p(ctx):
@@ -667,6 +695,24 @@ def test_training_step_in_a_graph(ctx, dtype):
             q, et, ew = chain(ctx, table, ids, w, target, weights, seed, dtype)
             assert all(torch.equal(a, b) for a, b in zip(r, q))
             assert torch.equal(dtable, et) and torch.equal(dw, ew)
+
+
+def test_gradient_of_a_column_in_a_graph(ctx):
+    """The path without a sort, captured and replayed on new ids."""
+    ids, grad = rand_ids(1, 40000, 30), rand(2, 40000, 24)
+    out = torch.zeros(30, 24, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        tokens.embed_grad(ctx, grad, ids, 30, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tokens.embed_grad(ctx, grad, ids, 30, out=out, accumulate=True)
+    ids.copy_(rand_ids(3, 40000, 30))
+    out.fill_(1.0)
+    graph.replay()
+    check_grad(out, grad, ids, 30, 1.0, torch.ones_like(out))
 
 
 def test_two_streams_at_once(ctx):
