@@ -943,6 +943,7 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaun
 // elements may lie in different rows; 1000000 x 7 f32: 16 us, 4.2 TB/s. magic = ceil(2^32 / classes): an element's row is the
 // high half of its index times magic, exactly, as index * classes < 2^32.
 constexpr uint32_t kGradRows = 1024;
+constexpr uint64_t kGradFewDepth = 8;  // 1000000 x 7 f32: 22.5 us; 4: 25.7 us, 2: 24.7 us, 1: 28.6 us
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGradLaunch a, uint32_t rows, uint32_t magic) {
@@ -1098,8 +1099,8 @@ cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, in
     const bool run = x % 16 == 0 && dx % 16 == 0 && (one || (a.ld_x == a.classes && a.ld_dx == a.classes));
     if (a.classes <= (run ? kGradFew : kGradFewStrided)) {
       const bool vec = run;
-      // about kGradDepth vectors a thread, whole vectors in whole rows
-      uint64_t rows = kGradThreads * kGradDepth * kV / a.classes;
+      // about kGradFewDepth vectors a thread, whole vectors in whole rows
+      uint64_t rows = kGradThreads * kGradFewDepth * kV / a.classes;
       rows = std::min<uint64_t>(std::max<uint64_t>(rows, 1) + kV - 1, kGradRows) / kV * kV;
       const uint64_t ctas = (a.n + rows - 1) / rows;
       if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;

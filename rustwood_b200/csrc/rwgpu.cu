@@ -895,13 +895,17 @@ extern "C" int rw_embed_device(rw_ctx* ctx, const void* d_table, int32_t table_t
 
 extern "C" int rw_embed_grad_workspace(rw_ctx* ctx, uint64_t n, uint64_t d, uint64_t vocab,
                                        uint64_t* bytes) {
-  if (!bytes) return fail(ctx, RW_ERR_ARG, "bytes is NULL");
-  *bytes = 0;
-  if (n > kMaxItems || vocab > kMaxItems || d > kMaxWidth)
-    return fail(ctx, RW_ERR_ARG,
-                "rw_embed_grad_workspace: n and vocab must be below 2^31, d below 2^23");
-  *bytes = embed_grad_workspace(n, d, vocab);
-  return RW_OK;
+  try {
+    if (!bytes) return fail(ctx, RW_ERR_ARG, "bytes is NULL");
+    *bytes = 0;
+    if (n > kMaxItems || vocab > kMaxItems || d > kMaxWidth)
+      return fail(ctx, RW_ERR_ARG,
+                  "rw_embed_grad_workspace: n and vocab must be below 2^31, d below 2^23");
+    *bytes = embed_grad_workspace(n, d, vocab);
+    return RW_OK;
+  } catch (...) {
+    return RW_ERR_OOM;
+  }
 }
 
 extern "C" int rw_embed_grad_device(rw_ctx* ctx, const void* d_grad, int32_t grad_type,
@@ -962,12 +966,16 @@ extern "C" int rw_dropout_device(rw_ctx* ctx, const void* d_x, int32_t type, uin
 
 extern "C" int rw_logprobs_workspace(rw_ctx* ctx, uint64_t n, uint64_t classes, int32_t type,
                                      uint32_t top_k, uint64_t* bytes) {
-  if (!bytes) return fail(ctx, RW_ERR_ARG, "bytes is NULL");
-  *bytes = 0;
-  if (!elem_type_ok(type) || top_k > RW_MAX_TOP || classes > kMaxItems)
-    return fail(ctx, RW_ERR_ARG, "rw_logprobs_workspace: bad type, top_k or classes");
-  *bytes = logprobs_workspace(n, classes, type, top_k);
-  return RW_OK;
+  try {
+    if (!bytes) return fail(ctx, RW_ERR_ARG, "bytes is NULL");
+    *bytes = 0;
+    if (!elem_type_ok(type) || top_k > RW_MAX_TOP || classes > kMaxItems)
+      return fail(ctx, RW_ERR_ARG, "rw_logprobs_workspace: bad type, top_k or classes");
+    *bytes = logprobs_workspace(n, classes, type, top_k);
+    return RW_OK;
+  } catch (...) {
+    return RW_ERR_OOM;
+  }
 }
 
 extern "C" int rw_logprobs_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n,
