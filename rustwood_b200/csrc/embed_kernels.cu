@@ -300,7 +300,7 @@ __device__ __forceinline__ uint64_t lower_bound(const unsigned long long* pairs,
 }
 
 template <typename TG, typename TD, int V>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads, V * sizeof(TG) >= 16 ? 4 : 1)
     k_embed_chunks(EmbedGradLaunch a, ChunkPlan cp, const unsigned long long* __restrict__ pairs,
                    float* __restrict__ partial, uint2* __restrict__ ends) {
   const uint32_t slot = threadIdx.x / cp.tx, lane = threadIdx.x % cp.tx;
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     k_embed_join(EmbedGradLaunch a, ChunkPlan cp, const float* __restrict__ partial,
                  const uint2* __restrict__ ends) {  // a chunk's first and last id
   constexpr int kWarps = kJoinThreads / 32;
-  constexpr uint32_t kLong = 24;  // chunks from which on a run is shared by the warps
+  constexpr uint32_t kLong = 12;  // chunks from which on a run is shared by the warps
   __shared__ uint32_t s_first[kJoinThreads], s_shared[kJoinThreads];  // runs; those all warps share
   __shared__ uint32_t s_count, s_long;
   __shared__ float4 s_part[kWarps][32];
@@ -848,7 +848,7 @@ ChunkPlan chunk_plan(uint64_t n, uint64_t d, int V) {
   c.pitch = (d + 3) / 4 * 4;
   c.join_lanes = 1;
   while (c.join_lanes < 32 && c.join_lanes * 4 < d) c.join_lanes *= 2;
-  const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * (c.tx >= 64 ? 16 : 4) * c.slots / c.col_blocks);
+  const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * (c.tx >= 64 ? 10 : 4) * c.slots / c.col_blocks);
   const uint64_t most = std::min<uint64_t>(want, 32768);
   c.chunk = (uint32_t)std::max<uint64_t>(8, (n + most - 1) / most);
   c.chunks = (uint32_t)((n + c.chunk - 1) / c.chunk);
