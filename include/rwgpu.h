@@ -319,8 +319,9 @@ int rw_embed_device(rw_ctx* ctx, const void* d_table, int32_t table_type, uint64
 
 /* Its gradient: dtable[v] = scale * (the sum of grad[i] over i with ids[i] == v), zero for
  * rows no id names; with accumulate != 0 the sums are added to the rows that ids name and
- * the other rows are left as they were. Sums are f32 in an order that ids, sizes, strides
- * and alignment fix, rounded once to dtable_type. Ids outside 0..vocab-1 have no gradient. n, vocab < 2^31,
+ * the other rows are left as they were. Sums are f32 in an order that ids, sizes and types
+ * fix (with at most 64 rows of at most 256 columns also grad's stride and alignment),
+ * rounded once to dtable_type. Ids outside 0..vocab-1 have no gradient. n, vocab < 2^31,
  * d < 2^23. */
 int rw_embed_grad_workspace(rw_ctx* ctx, uint64_t n, uint64_t d, uint64_t vocab, uint64_t* bytes);
 int rw_embed_grad_device(rw_ctx* ctx, const void* d_grad, int32_t grad_type, uint64_t ld_grad,

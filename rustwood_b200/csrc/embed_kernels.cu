@@ -827,28 +827,43 @@ cudaError_t launch_embed(const EmbedLaunch& a, cudaStream_t s, int* nl) {
 
 namespace {
 
-// Sizes and workspace offsets of one gradient call. The workspace covers either vector
-// width: it depends on n, d and vocab alone.
+// Sizes and workspace offsets of one gradient call. The workspace covers every type and
+// layout: it depends on n, d and vocab alone.
 struct GradPlan {
   uint64_t part;
   uint32_t parts, passes;
   uint64_t pairs0, pairs1, counts, partial, ends, bytes;  // offsets
 };
 
-// Chunks: enough for about 16 CTAs an SM where a row takes two warps or more, so that the
-// longest one does not decide the time; for narrower rows 4, whose slots are many and whose
-// runs then cross fewer chunks; no shorter than 8 positions (the partial sums would be more
-// than a quarter of the traffic) and no more than 32768 (k_embed_join looks at each).
-ChunkPlan chunk_plan(uint64_t n, uint64_t d, int V) {
-  ChunkPlan c = {};
+// How a row's d columns, V a thread, lie on CTAs.
+void chunk_columns(ChunkPlan& c, uint64_t d, int V) {
   c.dv = (d + V - 1) / V;
   c.tx = (uint32_t)std::min<uint64_t>(c.dv, kSumThreads);
   c.slots = kSumThreads / c.tx;
   c.col_blocks = (uint32_t)((c.dv + c.tx - 1) / c.tx);
+}
+
+// The columns a thread takes where no stride or base stands in the way: a 16-byte vector of
+// `elem`-byte elements, or what the width allows.
+int widest(uint64_t d, size_t elem) {
+  const int v = 16 / (int)elem;
+  return d % v == 0 ? v : d % 2 == 0 ? 2 : 1;
+}
+
+// Chunks: enough for about 10 CTAs an SM where a row takes two warps or more, so that the
+// longest one does not decide the time; for narrower rows 4, whose slots are many and whose
+// runs then cross fewer chunks; no shorter than 8 positions (the partial sums would be more
+// than a quarter of the traffic) and no more than 32768 (k_embed_join looks at each). Their
+// length follows n, d and the type's widest vectors, not the V that strides and bases leave, so
+// that the order of the sums does not depend on the layout.
+ChunkPlan chunk_plan(uint64_t n, uint64_t d, size_t elem, int V) {
+  ChunkPlan c = {};
+  chunk_columns(c, d, widest(d, elem));
+  const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * (c.tx >= 64 ? 10 : 4) * c.slots / c.col_blocks);
+  chunk_columns(c, d, V);
   c.pitch = (d + 3) / 4 * 4;
   c.join_lanes = 1;
   while (c.join_lanes < 32 && c.join_lanes * 4 < d) c.join_lanes *= 2;
-  const uint64_t want = std::max<uint64_t>(1, (uint64_t)kSms * (c.tx >= 64 ? 10 : 4) * c.slots / c.col_blocks);
   const uint64_t most = std::min<uint64_t>(want, 32768);
   c.chunk = (uint32_t)std::max<uint64_t>(8, (n + most - 1) / most);
   c.chunks = (uint32_t)((n + c.chunk - 1) / c.chunk);
@@ -893,9 +908,8 @@ GradPlan grad_plan(uint64_t n, uint64_t d, uint64_t vocab) {
   g.pairs0 = take(n * 8);
   g.pairs1 = take(n * 8);
   g.counts = take((uint64_t)g.parts * kRadix * 4);
-  const uint64_t chunks =
-      std::max({chunk_plan(n, d, 1).chunks, chunk_plan(n, d, 2).chunks, chunk_plan(n, d, 4).chunks,
-                chunk_plan(n, d, 8).chunks});
+  // they do not depend on V
+  const uint64_t chunks = std::max(chunk_plan(n, d, 2, 1).chunks, chunk_plan(n, d, 4, 1).chunks);
   g.partial = take(chunks * 2 * ((d + 3) / 4 * 4) * 4);
   g.ends = take(chunks * sizeof(uint2));
   // the table path keeps its CTAs' tables there instead
@@ -1012,7 +1026,7 @@ cudaError_t launch_embed_grad(const EmbedGradLaunch& a, void* workspace, cudaStr
                rw_packs(a.dtable, a.vocab, a.d, a.ld_dtable, sizeof(TD), V);
       };
       const int V = packs(kV) ? kV : packs(2) ? 2 : 1;
-      cp = chunk_plan(a.n, a.d, V);
+      cp = chunk_plan(a.n, a.d, sizeof(TG), V);
       // A zeroing CTA takes 128 KB, so that its search among the ids is a small part of it, or
       // more where that still leaves 32 an SM, so that the last ones do not decide the time.
       cp.zero_rows = (uint32_t)std::min<uint64_t>(

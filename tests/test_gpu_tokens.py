@@ -820,3 +820,15 @@ def test_strided_outputs_keep_what_lies_between(ctx):
         buf = torch.full((50, 3011), 7.0, device="cuda")
         call(buf[:, 5:3005])
         assert (buf[:, :5] == 7).all() and (buf[:, 3005:] == 7).all()
+
+
+@pytest.mark.parametrize("n,d,vocab", [(30000, 128, 300), (30000, 40, 2000), (9000, 264, 40), (3000, 96, 70)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_embed_grad_bits_do_not_depend_on_strides(ctx, n, d, vocab, dtype):
+    """The sums' order comes from ids, sizes and type where the ids are sorted."""
+    ids, grad = rand_ids(n, n, vocab), rand(n, n, d, dtype=dtype)
+    want = tokens.embed_grad(ctx, grad, ids, vocab)
+    out = strided(torch.zeros(vocab, d, device="cuda"), extra=5)
+    for g in (grad, strided(grad, extra=3), strided(grad, extra=1)):
+        assert torch.equal(tokens.embed_grad(ctx, g, ids, vocab), want)
+        assert torch.equal(tokens.embed_grad(ctx, g, ids, vocab, out=out), want)
