@@ -370,25 +370,23 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-// Elements 2 q and 2 q + 1 of a pack; CUT: not below kLowest.
+// Elements 2 q and 2 q + 1 of a pack; CUT: not below low (as bf16 has it).
 template <bool CUT, int V>
-__device__ __forceinline__ Two pair_of(const Pack<float, V>& p, int q) {
+__device__ __forceinline__ Two pair_of(const Pack<float, V>& p, int q, float low) {
   const float a = p.v[2 * q], b = p.v[2 * q + 1];
-  return CUT ? two_of(max_nan(a, kLowest), max_nan(b, kLowest)) : two_of(a, b);
+  return CUT ? two_of(max_nan(a, low), max_nan(b, low)) : two_of(a, b);
 }
 template <bool CUT, int V>
-__device__ __forceinline__ Two pair_of(const Pack<__nv_bfloat16, V>& p, int q) {
+__device__ __forceinline__ Two pair_of(const Pack<__nv_bfloat16, V>& p, int q, float low) {
   __nv_bfloat162 w = reinterpret_cast<const __nv_bfloat162*>(p.v)[q];
-  if (CUT) w = __hmax2_nan(w, __float2bfloat162_rn(kLowest));
+  if (CUT) w = __hmax2_nan(w, __float2bfloat162_rn(low));
   const uint32_t b = *reinterpret_cast<uint32_t*>(&w);
   return two_of(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
 }
 template <bool CUT, int V>
-__device__ __forceinline__ Two pair_of(const Pack<__half, V>& p, int q) {
-  // the lowest f16 above -inf is far above kLowest: only -inf is cut, to that
-  __half2 w = reinterpret_cast<const __half2*>(p.v)[q];
-  const float2 f = __half22float2(w);
-  return CUT ? two_of(max_nan(f.x, kLowest), max_nan(f.y, kLowest)) : two_of(f.x, f.y);
+__device__ __forceinline__ Two pair_of(const Pack<__half, V>& p, int q, float low) {
+  const float2 f = __half22float2(reinterpret_cast<const __half2*>(p.v)[q]);
+  return CUT ? two_of(max_nan(f.x, low), max_nan(f.y, low)) : two_of(f.x, f.y);
 }
 
 // The largest element of N packs, NaN if one is.
@@ -607,11 +605,17 @@ __device__ __forceinline__ float2 cta_sum(float2 v, float2 (&s_tmp)[W]) {
 // exactly and taken out of the sums at the end. A thread restates its sums only when a block
 // of kRowDepth vectors holds a new maximum.
 //
-// x * c must not overflow: margins below kLowest count as kLowest, and blocks whose maximum
-// so far is not above it are left out. That is exact where the row's maximum is in range;
-// where it is not (a row masked with the type's lowest value), and for scales far from 1, the
-// sums are taken again as e^{scale (x - m)}.
+// The rounding of m * c is up to half a unit in its last place, and 2 to that power is in the
+// sums until the end: it has to stay near 1, not only finite. So the sums hold where the row's
+// maximum is steady, |m c| below 2^22, where the rounding is at most 1/4; for a row or part
+// whose maximum is not (one masked with large finite numbers, margins of 1e7 and more), and for
+// scales far from 1, they are taken again as e^{scale (x - m)}. Under a steady maximum margins at
+// or below -2^23 / c have e^{scale (x - m)} = 0: they count as that, and blocks whose maximum so
+// far is not above it are left out, so that no exponent on the way passes 2^24 in size.
 // ENT: with the entropy's sum.
+constexpr float kSteady = 4194304.0f;  // 2^22
+__device__ __forceinline__ bool steady(float m, float c) { return fabsf(m) * c < kSteady; }
+__device__ __forceinline__ float lowest_of(float c) { return __fdividef(-2.0f * kSteady, c); }
 __device__ __forceinline__ bool in_range(float m) { return m > kLowest && m < -kLowest; }
 __device__ __forceinline__ bool scale_in_range(float s) { return s >= 1e-6f && s <= 1e6f; }
 
@@ -628,7 +632,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
   const uint64_t lo = part * sr.part, hi = min(lo + sr.part, a.classes);
   const Span<T> sp((const T*)a.x + i * a.ld_x + lo, (uint32_t)(hi - lo));
   rw_let_successor_start();  // k_logprobs_join of a split row waits for this kernel
-  const float c = a.scale * kLog2e;
+  const float c = a.scale * kLog2e, low = lowest_of(c);
   const int64_t target = t == 0 && sr.parts == 1 ? target_of(a, i) : -1;
 
   float m = -kInf, mc = 0.0f;
@@ -639,7 +643,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
     if (!(top <= m)) {
       top = max_nan(top, m);
       const float next = top * c;
-      if (m > kLowest) {
+      if (m > low) {
         const float d = mc - next, f = exp2_fast(max_nan(d, kLowest));
         const Two f2 = two_of(f, f), zero = 0;
         if (ENT) w = fma2(f2, fma2(two_of(d, d), s, w), zero);
@@ -649,12 +653,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
       mc = next;
       base = two_of(-next, -next);
     }
-    if (m <= kLowest) return;
+    if (m <= low) return;
 #pragma unroll
     for (int u = 0; u < kCount; u++) {
 #pragma unroll
       for (int q = 0; q < kV / 2; q++) {
-        const Two d = fma2(pair_of<ENT>(p[u], q), c2, base);
+        const Two d = fma2(pair_of<ENT>(p[u], q, low), c2, base);
         const float2 df = both(d);
         const Two e = two_of(exp2_fast(df.x), exp2_fast(df.y));
         s = add2(s, e);
@@ -701,7 +705,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
   const float at_target = margin_at<T>(a, i, target, in_row);
   Sums r;
   r.m = m;
-  if (!(m <= kLowest)) {
+  if (!(m <= low)) {
     // the sums are those of e^{scale (x - m)} times 2^off
     const float off = __fmaf_rn(m, c, -mc), f = exp2_fast(-off);
     const float2 sf = both(s), wf = both(w);
@@ -719,7 +723,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs_row(LogprobsLaunch a
   const float all = cta_max(own, s_max);
   if (a.top_k) top_groups(s_top);
   if (all != -kInf) {
-    if (!(in_range(all) && scale_in_range(a.scale))) {
+    if (!(steady(all, c) && scale_in_range(a.scale))) {
       r.s = r.t = 0.0f;
       for (uint32_t j = t; j < sp.n; j += kRowThreads) {
         const float d = max_nan(rw_widen(sp.x[j]) - all, kLowest), e = exp2_fast(d * c);
@@ -924,7 +928,7 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaun
     if (r.kind == 1 && v != hit) {
 #pragma unroll
       for (int q = 0; q < kV / 2; q++) {
-        const Two d = fma2(pair_of<ENT>(p[u], q), c2, k2);
+        const Two d = fma2(pair_of<ENT>(p[u], q, kLowest), c2, k2);
         const float2 df = both(d), w = ENT ? both(fma2(b2, d, a2)) : make_float2(-r.a, -r.a);
         p[u].set(2 * q, exp2_fast(df.x) * w.x);
         p[u].set(2 * q + 1, exp2_fast(df.y) * w.y);
@@ -993,7 +997,7 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGrad
         const Two c2 = two_of(c, c), k2 = two_of(-r.x, -r.x), a2 = two_of(-r.y, -r.y), b2 = two_of(-r.z, -r.z);
 #pragma unroll
         for (int q = 0; q < kV / 2; q++) {
-          const Two d = fma2(pair_of<true>(p, q), c2, k2);
+          const Two d = fma2(pair_of<true>(p, q, kLowest), c2, k2);
           const float2 df = both(d), w = both(fma2(b2, d, a2));
           p.set(2 * q, target == -2 ? 0.0f : exp2_fast(df.x) * w.x);
           p.set(2 * q + 1, target == -2 ? 0.0f : exp2_fast(df.y) * w.y);

@@ -832,3 +832,41 @@ def test_embed_grad_bits_do_not_depend_on_strides(ctx, n, d, vocab, dtype):
     for g in (grad, strided(grad, extra=3), strided(grad, extra=1)):
         assert torch.equal(tokens.embed_grad(ctx, g, ids, vocab), want)
         assert torch.equal(tokens.embed_grad(ctx, g, ids, vocab, out=out), want)
+
+
+def far_rows(v, dtype, scale):
+    """Rows whose margins are far from 0 in units of 1 / scale, wholly or in part."""
+    at = torch.arange(v, device="cuda")
+    x, _ = margins(v, 1, v, dtype)
+    x = x.float()[0]
+    rows = []
+    for mask in (-1e9, -1e10, -1e12, -1e18, -1e20, -1e29, -9e29, -1e31):
+        rows.append(torch.full_like(x, mask))
+        rows.append(torch.where(at < v * 3 // 4, mask, x))            # the first classes masked
+        rows.append(torch.where(at // 8 % 256 < 200, mask, x))        # long runs, whole threads' shares
+        rows.append(torch.where(at == v // 2, -mask, x))              # one far above
+    level = at.remainder(3).float()
+    for top in (1e4, 2.9e6, 3.0e6, 2.3e7, 1.1e9, 1e10, -1e4, -2.9e6, -3.1e6, -1e10):
+        near = top / scale
+        rows.append(near + level * abs(near) * 2.0 ** -7)             # steps that every type has
+        rows.append(near + (at == v - 1).float() * abs(near))         # one class ahead at the end
+    rows = torch.stack(rows)
+    if dtype == F16:
+        rows = rows.clamp(-65504, 65504)
+    return rows.to(dtype)
+
+
+@pytest.mark.parametrize("v", [7, 100, 900, 1500, 30000, 140000])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_logprobs_of_far_finite_margins(ctx, v, dtype):
+    """Masks by finite numbers, offsets shared by a row, scales that make margins far."""
+    for scale in (1.0, 2.0 ** -10, 1e3, 1e6):
+        x = far_rows(v, dtype, scale)
+        t = torch.arange(len(x), device="cuda") * 977 % v
+        got = tokens.logprobs(ctx, x, t, scale=scale, top_k=2)
+        check_logprobs(got, x, t, scale, 2)
+        other = tokens.logprobs(ctx, strided(x), t, scale=scale)
+        check_logprobs(other, x, t, scale, 0)
+        if v in (1500, 30000):  # rows enough that none is split
+            many = tokens.logprobs(ctx, x.repeat(12, 1), t.repeat(12), scale=scale, top_k=2)
+            check_logprobs(type(many)(*(f[-len(x):] for f in many)), x, t, scale, 2)
