@@ -616,7 +616,6 @@ __device__ __forceinline__ float2 cta_sum(float2 v, float2 (&s_tmp)[W]) {
 constexpr float kSteady = 4194304.0f;  // 2^22
 __device__ __forceinline__ bool steady(float m, float c) { return fabsf(m) * c < kSteady; }
 __device__ __forceinline__ float lowest_of(float c) { return __fdividef(-2.0f * kSteady, c); }
-__device__ __forceinline__ bool in_range(float m) { return m > kLowest && m < -kLowest; }
 __device__ __forceinline__ bool scale_in_range(float s) { return s >= 1e-6f && s <= 1e6f; }
 
 template <typename T, bool ENT, int NT>
@@ -826,7 +825,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
 // =================================================================================
 // The gradient: elementwise, as dx = hit - 2^d (A + B d) with d = x * c - K and the row's
 // constants K = m c + log_sum log2(e), A, B and (at the target) hit. K is rounded to f32 and
-// what the rounding dropped is a factor of A and B, so large margins lose nothing.
+// what the rounding dropped, at most 1/2 where m is steady, is a factor of A and B. Rows whose
+// maximum is not steady are computed by the formula, from x - m.
 
 constexpr int kGradThreads = 256;
 constexpr int kGradDepth = 4;
@@ -850,13 +850,14 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobsGradLaunch& a, uint64_
   }
   const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f;
   if (g == 0.0f && e == 0.0f) return r;
-  if (!(in_range(m) && scale_in_range(a.scale))) {  // the constants could overflow
+  const float c = a.scale * kLog2e;
+  if (!(steady(m, c) && scale_in_range(a.scale))) {
     r.kind = 2;
     return r;
   }
   // k = m c + log_sum log2(e) in two f32: products and sum with their roundings
   constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
-  const float c = a.scale * kLog2e, s = a.log_sum[i];
+  const float s = a.log_sum[i];
   const float mc = m * c, sl = s * kLog2e;
   const float k = mc + sl, back = k - mc;
   const float rest = ((mc - (k - back)) + (sl - back)) +

@@ -870,3 +870,33 @@ def test_logprobs_of_far_finite_margins(ctx, v, dtype):
         if v in (1500, 30000):  # rows enough that none is split
             many = tokens.logprobs(ctx, x.repeat(12, 1), t.repeat(12), scale=scale, top_k=2)
             check_logprobs(type(many)(*(f[-len(x):] for f in many)), x, t, scale, 2)
+
+
+def check_scaled_grad(got, *args):
+    """check_logprobs_grad for gradients that a 16-bit type may not hold: near its largest number
+    and beyond, only the sign and that it is large. Probabilities below 2^-126, f32's smallest
+    normal number, may count as 0; there |log p| is near 88 (where it is above 100, what is lost
+    is less still), so that loses at most 2^-126 (|g| + |e| (100 + h)) scale."""
+    want, tol = grad_of_logprobs(*args)
+    h, g, e, scale = args[4:]
+    tol = tol + (scale * 2.0 ** -126 * (g.double().abs() + e.double().abs() * (100 + h.double().abs())))[:, None]
+    large = want.abs() > torch.finfo(got.dtype).max * 0.98
+    tol = tol + half_step(got.dtype) * (want.abs() + tol) + (2.0 ** -25 if got.dtype == F16 else 1e-37)
+    off = (got.double() - want).abs()
+    assert (large | (off <= tol)).all(), float((off - tol)[~large].max())
+    assert ((got.double() * want.sign()) >= torch.finfo(got.dtype).max * 0.95)[large].all()
+
+
+@pytest.mark.parametrize("v", [7, 100, 900, 1500, 30000, 140000])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_logprobs_grad_of_far_finite_margins(ctx, v, dtype):
+    for scale in (1.0, 2.0 ** -10, 1e3):
+        x = far_rows(v, dtype, scale)
+        t = torch.arange(len(x), device="cuda") * 977 % v
+        m, log_sum, _, _, h = (f.float() for f in logprob_reference(x, t, scale, 0)[:5])
+        g, e = -torch.ones(len(x), device="cuda"), torch.full((len(x),), 0.5, device="cuda")
+        for out in (torch.zeros_like(x), strided(torch.zeros_like(x))):
+            tokens.logprobs_grad(ctx, x, t, m, log_sum, h, g, e, scale=scale, out=out)
+            check_scaled_grad(out, x, t, m, log_sum, h, g, e, scale)
+        got = tokens.logprobs_grad(ctx, x, t, m, log_sum, None, g, scale=scale)
+        check_scaled_grad(got, x, t, m, log_sum, h, g, torch.zeros_like(g), scale)
