@@ -828,6 +828,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_logprobs_join(LogprobsLaunch a
 // what the rounding dropped, at most 1/2 where m is steady, is a factor of A and B. Rows whose
 // maximum is not steady are computed by the formula, from x - m.
 
+// Margins below it count as it. A steady maximum at a scale in range is above -3e12, so 2^d is 0
+// there, and d, at least -2e13 c, leaves A + B d finite for every A and B in use.
+constexpr float kGradLowest = -1e13f;
+
 constexpr int kGradThreads = 256;
 constexpr int kGradDepth = 4;
 
@@ -869,21 +873,22 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobsGradLaunch& a, uint64_
   r.a = f * (g + e * (h - rest * kLn2));
   r.b = f * e * kLn2;
   r.hit = g * a.scale;
-  r.kind = 1;
+  r.kind = fabsf(r.a) < 1e30f && fabsf(r.b) * c < 1e24f ? 1 : 2;  // A + B d stays finite
   return r;
 }
-// One element by the formula.
+// One element by the formula. p is multiplied first: where it is 0 nothing else may overflow.
 __device__ __forceinline__ float grad_of(const LogprobsGradLaunch& a, uint64_t i, float x, bool hit, bool in) {
   const float lp = max_nan((x - a.row_max[i]) * a.scale - a.log_sum[i], kLowest);
   const float g = in ? a.grad_logp[i] : 0.0f;
   const float e = a.grad_entropy ? a.grad_entropy[i] : 0.0f, h = a.grad_entropy ? a.entropy[i] : 0.0f;
-  return ((hit ? g : 0.0f) - exp2_fast(lp * kLog2e) * (g + e * (lp + h))) * a.scale;
+  const float p = exp2_fast(lp * kLog2e);
+  return ((hit ? g : 0.0f) - (p * g + e * (p * (lp + h)))) * a.scale;
 }
 __device__ __forceinline__ float grad_element(const LogprobsGradLaunch& a, uint64_t i, const RowGrad& r, float c,
                                               float x, uint32_t j) {
   const bool hit = (int32_t)j == r.target;
   if (r.kind == 2) return grad_of(a, i, x, hit, r.target >= 0);
-  const float d = __fmaf_rn(max_nan(x, kLowest), c, -r.k);
+  const float d = __fmaf_rn(max_nan(x, kGradLowest), c, -r.k);
   const float v = -exp2_fast(d) * __fmaf_rn(r.b, d, r.a);
   return hit ? v + r.hit : v;
 }
@@ -892,7 +897,7 @@ __device__ __forceinline__ float grad_element(const LogprobsGradLaunch& a, uint6
 // same distance from a 16-byte boundary (VEC), else it goes element by element. 4096 x 128000
 // bf16 with entropy: 383 us, 5.5 TB/s, bound by the memory's mixed reads and writes.
 template <typename T, bool VEC, bool ENT>
-__global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaunch a, uint32_t chunks) {
+__global__ void __launch_bounds__(kGradThreads, sizeof(T) == 2 ? 6 : 5) k_logprobs_grad(LogprobsGradLaunch a, uint32_t chunks) {
   constexpr int kV = Span<T>::kV;
   const uint64_t i = blockIdx.x / chunks;
   const uint32_t chunk = blockIdx.x % chunks, t = threadIdx.x;
@@ -929,7 +934,7 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad(LogprobsGradLaun
     if (r.kind == 1 && v != hit) {
 #pragma unroll
       for (int q = 0; q < kV / 2; q++) {
-        const Two d = fma2(pair_of<ENT>(p[u], q, kLowest), c2, k2);
+        const Two d = fma2(pair_of<ENT>(p[u], q, kGradLowest), c2, k2);
         const float2 df = both(d), w = ENT ? both(fma2(b2, d, a2)) : make_float2(-r.a, -r.a);
         p[u].set(2 * q, exp2_fast(df.x) * w.x);
         p[u].set(2 * q + 1, exp2_fast(df.y) * w.y);
@@ -952,7 +957,7 @@ constexpr uint64_t kGradFewDepth = 8;  // 1000000 x 7 f32: 22.5 us; 4: 25.7 us, 
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGradLaunch a, uint32_t rows, uint32_t magic) {
-  __shared__ float4 s_row[kGradRows];     // k, a, b, hit
+  __shared__ float4 s_row[kGradRows];     // k (NaN: by the formula), a, b, hit
   __shared__ int32_t s_target[kGradRows];  // -1: none, -2: a row of zeros
   constexpr int kV = VEC ? 16 / (int)sizeof(T) : 1;
   const uint64_t first = (uint64_t)blockIdx.x * rows;
@@ -964,7 +969,7 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGrad
   bool formula = false;
   for (uint32_t k = threadIdx.x; k < count; k += kGradThreads) {
     const RowGrad r = row_grad(a, first + k);
-    s_row[k] = make_float4(r.k, r.a, r.b, r.hit);
+    s_row[k] = make_float4(r.kind == 2 ? NAN : r.k, r.a, r.b, r.hit);
     s_target[k] = r.kind ? r.target : -2;
     formula |= r.kind == 2;
   }
@@ -974,31 +979,36 @@ __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGrad
     const float4 r = s_row[row];
     const int32_t target = s_target[row];
     const bool hit = (int32_t)j == target;
-    float v;
-    if (formula) {  // every row of the CTA, by the row's own rule
-      v = target == -2 ? 0.0f : grad_element(a, first + row, row_grad(a, first + row), c, in, j);
-    } else {
-      const float d = __fmaf_rn(max_nan(in, kLowest), c, -r.x);
-      v = -exp2_fast(d) * __fmaf_rn(r.z, d, r.y);
-      v = hit ? v + r.w : v;
-      v = target == -2 ? 0.0f : v;
-    }
-    return v;
+    const float d = __fmaf_rn(max_nan(in, kGradLowest), c, -r.x);
+    float v = -exp2_fast(d) * __fmaf_rn(r.z, d, r.y);
+    v = hit ? v + r.w : v;
+    return target == -2 ? 0.0f : v;
   };
   auto row_of = [&](uint32_t at) { return classes == 1 ? at : __umulhi(at, magic); };
+  if (formula) {  // element by element, every row by its own rule
+    for (uint32_t at = threadIdx.x; at < total; at += kGradThreads) {
+      const uint32_t row = row_of(at), j = at - row * classes;
+      const int32_t target = s_target[row];
+      const float in = rw_widen(x[row * a.ld_x + j]);
+      const bool by_formula = s_row[row].x != s_row[row].x;
+      dx[row * a.ld_dx + j] = rw_round<T>(
+          by_formula ? grad_of(a, first + row, in, (int32_t)j == target, target >= 0) : element(at, row, in));
+    }
+    return;
+  }
   for (uint32_t j0 = threadIdx.x * kV; j0 < total; j0 += kGradThreads * kV) {
     if (VEC && j0 + kV <= total) {
       Pack<T, kV> p;
       p.load(x + j0);
       const uint32_t row = row_of(j0), j = j0 - row * classes;
       const int32_t target = s_target[row];
-      if (kV > 1 && classes >= 16 * kV && !formula && j + kV <= classes && (uint32_t)(target - (int32_t)j) >= kV) {
+      if (kV > 1 && classes >= 16 * kV && j + kV <= classes && (uint32_t)(target - (int32_t)j) >= kV) {
         // one row's, and the target elsewhere
         const float4 r = s_row[row];
         const Two c2 = two_of(c, c), k2 = two_of(-r.x, -r.x), a2 = two_of(-r.y, -r.y), b2 = two_of(-r.z, -r.z);
 #pragma unroll
         for (int q = 0; q < kV / 2; q++) {
-          const Two d = fma2(pair_of<true>(p, q, kLowest), c2, k2);
+          const Two d = fma2(pair_of<true>(p, q, kGradLowest), c2, k2);
           const float2 df = both(d), w = both(fma2(b2, d, a2));
           p.set(2 * q, target == -2 ? 0.0f : exp2_fast(df.x) * w.x);
           p.set(2 * q + 1, target == -2 ? 0.0f : exp2_fast(df.y) * w.y);

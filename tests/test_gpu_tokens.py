@@ -900,3 +900,43 @@ def test_logprobs_grad_of_far_finite_margins(ctx, v, dtype):
             check_scaled_grad(out, x, t, m, log_sum, h, g, e, scale)
         got = tokens.logprobs_grad(ctx, x, t, m, log_sum, None, g, scale=scale)
         check_scaled_grad(got, x, t, m, log_sum, h, g, torch.zeros_like(g), scale)
+
+
+@pytest.mark.parametrize("scale", [1.0, 30.0, 1e3, 1e5, 1e6, 1e12])
+@pytest.mark.parametrize("v", [7, 600, 5000, 9001])
+def test_entropy_gradient_of_masked_classes_at_large_scales(ctx, v, scale):
+    """Few and many classes, by vectors and element by element (a dx that lies differently);
+    margins of order 1 / scale, so that many classes count, and of order 1."""
+    for dtype in TYPES:
+        x, t = margins(v, 6, v, dtype, std=2.0)
+        x[:4] = (x[:4].float() / scale).to(dtype)
+        t = torch.tensor([v - 1, -1, 2, v - 1, 1, v - 1], device="cuda")
+        x[0, : v // 2] = -INF
+        x[1, 1:] = -INF
+        x[2, 1::2] = -INF
+        x[4, 2:] = -INF
+        x[5, ::3] = -INF
+        m, log_sum, _, _, h = (f.float() for f in logprob_reference(x, t, scale, 0)[:5])
+        g = -torch.ones(6, device="cuda")
+        gone = x == -INF
+        gone[torch.arange(6, device="cuda"), t] = False
+        for e in (torch.full((6,), 1e-2, device="cuda"), torch.full((6,), -655.0, device="cuda")):
+            for out in (torch.zeros_like(x), strided(torch.zeros_like(x))):
+                tokens.logprobs_grad(ctx, x, t, m, log_sum, h, g, e, scale=scale, out=out)
+                check_scaled_grad(out, x, t, m, log_sum, h, g, e, scale)
+                assert (out[gone] == 0).all()
+                tokens.logprobs_grad(ctx, x, None, m, log_sum, h, None, e, scale=scale, out=out)
+                check_scaled_grad(out, x, t, m, log_sum, h, torch.zeros_like(g), e, scale)
+
+
+@pytest.mark.parametrize("v", [7, 900, 30000])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_logprobs_grad_of_far_finite_margins_at_a_large_scale(ctx, v, dtype):
+    scale = 1e6
+    x = far_rows(v, dtype, scale)
+    t = torch.arange(len(x), device="cuda") * 977 % v
+    m, log_sum, _, _, h = (f.float() for f in logprob_reference(x, t, scale, 0)[:5])
+    g, e = -torch.ones(len(x), device="cuda"), torch.full((len(x),), 0.5, device="cuda")
+    for out in (torch.zeros_like(x), strided(torch.zeros_like(x))):
+        tokens.logprobs_grad(ctx, x, t, m, log_sum, h, g, e, scale=scale, out=out)
+        check_scaled_grad(out, x, t, m, log_sum, h, g, e, scale)
