@@ -550,12 +550,12 @@ __device__ void top_places(const Span<T>& sp, uint32_t offset, float own, uint32
   }
   // The largest margins are more than the candidates' space and lie in few groups: place by
   // place over the whole span.
-  Key last = ~0ull;
+  Key last = 0;  // that of the place before
   for (uint32_t place = 0; place < top_k; place++) {
     Key best = 0;
     for (uint32_t j = t; j < sp.n; j += kRowThreads) {
       const Key k = key_of(order_of(rw_widen(sp.x[j])), offset + j);
-      if (k < last && k > best) best = k;
+      if ((place == 0 || k < last) && k > best) best = k;  // a NaN of class 0 has the largest key
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));

@@ -940,3 +940,18 @@ def test_logprobs_grad_of_far_finite_margins_at_a_large_scale(ctx, v, dtype):
     for out in (torch.zeros_like(x), strided(torch.zeros_like(x))):
         tokens.logprobs_grad(ctx, x, t, m, log_sum, h, g, e, scale=scale, out=out)
         check_scaled_grad(out, x, t, m, log_sum, h, g, e, scale)
+
+
+def test_nan_at_the_first_class_ranks_first(ctx):
+    """Also where the largest margins are more than are kept as candidates, in few threads."""
+    v, k = 140000, 5
+    x, _ = margins(1, 1, v, F32)
+    at = torch.arange(v, device="cuda")
+    x[0] += torch.where(at // 4 % 256 < 4, 30.0, 0.0)
+    want = torch.sort(x[0], descending=True, stable=True).indices[:k]
+    want = torch.cat([want.new_zeros(1), want[want != 0]])[:k]
+    x[0, 0] = NAN
+    for n in (1, 600):
+        got = tokens.logprobs(ctx, x.expand(n, v).contiguous(), top_k=k)
+        assert torch.equal(got.top_index, want.expand(n, k))
+        assert got.top_logp.isnan().all()
