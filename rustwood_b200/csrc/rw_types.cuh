@@ -106,26 +106,6 @@ inline cudaError_t rw_with_index(int type, F f) {
   return cudaErrorInvalidValue;
 }
 
-// A load of read-only global memory that stays where it is written: the compiler does not
-// sink a batch of them to their uses, so they are in flight together.
-template <typename T>
-__device__ __forceinline__ T rw_load_here(const T* p) {
-  if constexpr (sizeof(T) == 2) {
-    uint16_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
-    return *reinterpret_cast<T*>(&v);
-  } else if constexpr (sizeof(T) == 4) {
-    uint32_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return *reinterpret_cast<T*>(&v);
-  } else {
-    static_assert(sizeof(T) == 8, "2, 4 or 8 bytes");
-    uint64_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u64 %0, [%1];" : "=l"(v) : "l"(p));
-    return *reinterpret_cast<T*>(&v);
-  }
-}
-
 // Programmatic dependent launch: a kernel launched as `dependent` (rw_launch) lets its
 // successor start, then waits until its predecessors' writes are visible.
 __device__ __forceinline__ void rw_let_successor_start() {
