@@ -349,6 +349,9 @@ int rw_dropout_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t rows,
  *   top_index / top_logp [n][top_k]: the top_k <= min(RW_MAX_TOP, classes) largest margins
  *            in descending order, the lower index first among equal ones, and their logp.
  * All outputs are f32 (top_index int64) and nullable; d_targets is needed with d_logp only.
+ * log_sum and entropy, and what log_sum adds to the others, are right absolutely, to the
+ * rounding of an f32 sum that holds the maximum's 1: in a row whose other classes have less
+ * than 2^-24 together log_sum is 0.
  * A row whose margins are all -inf has row_max, lse, logp and top_logp -inf, log_sum and
  * entropy 0. A NaN or +inf among the margins makes log_sum, lse, logp, entropy and top_logp
  * NaN; NaN ranks above +inf. classes < 2^31. */
@@ -364,7 +367,10 @@ int rw_logprobs_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n, u
  * respect to the margins, from rw_logprobs_device's row_max, log_sum and (with
  * d_grad_entropy) entropy. d_targets with d_grad_logp, and d_grad_entropy, are each
  * nullable. A target outside 0..classes-1 contributes nothing; a row whose row_max is -inf,
- * or whose grad_logp and grad_entropy are both zero or absent, has a gradient of zeros. dx has the margins' type and may be x (with the same stride). */
+ * or whose grad_logp and grad_entropy are both zero or absent, has a gradient of zeros.
+ * Probabilities, 1 - p at the target among them, are right to about 2^-21 absolutely, and
+ * those below 2^-126 count as 0. dx has the margins' type and may be x (with the same
+ * stride). */
 int rw_logprobs_grad_device(rw_ctx* ctx, const void* d_x, int32_t type, uint64_t n,
                             uint64_t classes, uint64_t ld_x, float scale, const void* d_targets,
                             int32_t target_type, const float* d_row_max, const float* d_log_sum,

@@ -24,8 +24,9 @@ constexpr int kSms = 148;
 
 // `tx` threads a row, V columns a thread and access; a thread takes R rows and C vectors of
 // each at a time, all in flight, so that short rows have as much in flight as long ones. Every
-// CTA takes slots * R rows and is done. 65536 x 4096 bf16: 131 us, 5.3 TB/s of the bytes that
-// have to move; 136 us with a resident grid, 167 us with two vectors in flight.
+// CTA takes slots * R rows and is done. 65536 x 4096 bf16: 129 us, 5.4 TB/s of the bytes that
+// have to move; 136 us with a resident grid, 167 us with two vectors in flight. Odd widths of
+// 16-bit rows go two bytes at a time (30000 x 2001 bf16 93 us, x 2002 40 us, x 2048 31 us).
 constexpr int kEmbedThreads = 256;
 
 struct EmbedPlan {
@@ -265,8 +266,10 @@ __global__ void __launch_bounds__(kCountThreads)
 // an f32 partial sum in each of them, and k_embed_join adds those in the chunks' order. So
 // a frequent id is summed by many slots, and the order of every addition is fixed by the
 // ids and the sizes. Rows that no id names are zeroed by further CTAs of the same launch.
-// 65536 x 4096 bf16 into 128000 rows f32: 441 us for 2.6 GB, 6.0 TB/s; 482 us with the sort
-// and the join.
+// 65536 x 4096 bf16 into 128000 rows f32: 438 us for 2.6 GB, 5.9 TB/s; 473 us with the sort
+// and the join. Four CTAs an SM, as its launch bounds ask for, against two that 78 registers
+// leave: 36548 x 1128 bf16 into 8 rows 50 us and 54 us, 200000 x 1024 into 100 119 us and 127 us
+// (a 60000 x 502, whose vectors are narrow, takes 75 us either way).
 
 constexpr int kSumThreads = 256;
 constexpr int kSumDepth = 4;    // rows in flight per thread
@@ -400,7 +403,9 @@ __global__ void __launch_bounds__(kJoinThreads)
     k_embed_join(EmbedGradLaunch a, ChunkPlan cp, const float* __restrict__ partial,
                  const uint2* __restrict__ ends) {  // a chunk's first and last id
   constexpr int kWarps = kJoinThreads / 32;
-  constexpr uint32_t kLong = 12;  // chunks from which on a run is shared by the warps
+  // Chunks from which on a run is shared by the warps (24: 500000 x 64 f32 into 50000 rows 111 us
+  // instead of 103 us, 60000 x 502 bf16 into 30000 78 us instead of 75 us).
+  constexpr uint32_t kLong = 12;
   __shared__ uint32_t s_first[kJoinThreads], s_shared[kJoinThreads];  // runs; those all warps share
   __shared__ uint32_t s_count, s_long;
   __shared__ float4 s_part[kWarps][32];
@@ -504,8 +509,12 @@ __global__ void __launch_bounds__(kJoinThreads)
 // of grad once, in memory order, through a ring of tiles in shared memory that asynchronous
 // copies fill; a ninth warp turns the ids into offsets, so that a sum is two loads, an
 // addition and a store. 1000003 x 33 f32 into 50 rows: 42 us, the shared-memory pipe busy for
-// three quarters of it; 51 us with loads to registers, 156 us by sorting, whose walk reads
-// rows of 132 bytes in category order. grad has to be contiguous and aligned.
+// three quarters of it; 51 us with loads to registers, 130 us by sorting, whose walk reads
+// rows of 132 bytes in category order. grad has to be contiguous and aligned. 300000 x 16 f32
+// into 64 rows: 12 us, 55 us by sorting; 100000 x 256 bf16 into 30: 29 us and 45 us; 2000 x 16
+// into 50: 6 us and 12 us. 64 rows is where shared memory is still cheap, not where the two
+// meet: with 96, 1000003 x 33 f32 would take 60 us here and 129 us sorted, but 100000 x 256 bf16
+// 45 us here and 42 us sorted.
 constexpr uint32_t kTableRows = 64;
 constexpr uint32_t kTableCols = kSumThreads;
 constexpr int kTableStages = 4;
@@ -718,9 +727,10 @@ constexpr int kDropoutDepth = 8 / (int)sizeof(T);  // 64 bytes
 
 // One thread takes the 8 elements of a counter, kDropoutDepth counters whose loads are all in
 // flight before it computes, and is done: many short CTAs overlap better than a resident grid
-// that walks the matrix with as many loads in flight (268M bf16: 185 us, 5.8 TB/s, against
+// that walks the matrix with as many loads in flight (268M bf16: 182 us, 5.9 TB/s, against
 // 209-221 us). VEC: the matrices are contiguous and 16-byte aligned, so a group is one or two
-// 16-byte accesses; the last, partial one goes element by element.
+// 16-byte accesses; the last, partial one goes element by element. Other layouts do throughout:
+// 65536 x 1024 bf16 45 us contiguous, 231 us strided.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256, kDropoutCtas) k_dropout(DropoutLaunch a, PhiloxKeys keys) {
   const uint64_t total = a.rows * a.cols;
@@ -782,7 +792,8 @@ cudaError_t embed_launch(const EmbedLaunch& a, cudaStream_t s) {
   EmbedPlan ep;
   ep.dv = (uint32_t)(a.d / V);
   // few rows: a vector a thread, a row's columns over several CTAs; many: four a thread, of one
-  // row where a row has four warps' worth, else of two or four rows
+  // row where a row has four warps' worth, else of two or four rows. Rows of 256 bf16, few and
+  // many: 600 of them 2.0 us and 2.5 us; of 4096: 2400 of them 9.1 us and 8.2 us.
   const bool many = a.n >= 8 * kSms;
   const uint32_t warps = (ep.dv + 31) / 32;
   int c = !many ? 1 : warps >= 4 ? 4 : warps >= 2 ? 2 : 1;
@@ -851,7 +862,9 @@ int widest(uint64_t d, size_t elem) {
 }
 
 // Chunks: enough for about 10 CTAs an SM where a row takes two warps or more, so that the
-// longest one does not decide the time; for narrower rows 4, whose slots are many and whose
+// longest one does not decide the time (16: 36548 x 1128 bf16 into 8 rows 59 us instead of 50 us,
+// 65536 x 4096 bf16 into 128000 481 us instead of 475 us, f32 498 us instead of 506 us); for
+// narrower rows 4, whose slots are many and whose
 // runs then cross fewer chunks; no shorter than 8 positions (the partial sums would be more
 // than a quarter of the traffic) and no more than 32768 (k_embed_join looks at each). Their
 // length follows n, d and the type's widest vectors, not the V that strides and bases leave, so

@@ -5,7 +5,9 @@
 //   logp_t  = d_t - log_sum                      entropy = log_sum - (sum_j e^{d_j} d_j) / s
 //
 // and the k largest margins (the lower index first among equal ones) with their logp.
-// Both terms of the entropy have one sign, so it loses nothing to cancellation. A row whose
+// Both terms of the entropy have one sign, so no digits cancel between them. s holds the
+// maximum's own 1: log_sum, and with it logp and entropy, are right absolutely, to the rounding of
+// that sum, and other classes that have less than 2^-24 together do not count. A row whose
 // margins are all -inf has m = lse = logp = -inf, log_sum = entropy = 0; a NaN or +inf among
 // the margins makes the row's outputs NaN (m is what it is).
 //
@@ -599,8 +601,8 @@ __device__ __forceinline__ float2 cta_sum(float2 v, float2 (&s_tmp)[W]) {
 }
 
 // One pass over a row (or part): 16-byte vectors, kRowDepth in flight beside the kRowDepth that
-// are being summed (4096 x 128000 bf16 with entropy and top 5: 204 us, 5.1 TB/s; 337 us without
-// the second buffer), exponents as one
+// are being summed (4096 x 128000 bf16 with entropy and top 5: 185 us alone, 5.7 TB/s of the bytes
+// that have to move; 337 us without the second buffer), exponents as one
 // fused multiply-add e = x * c - mc with mc = round(m * c); the rounding of mc is known
 // exactly and taken out of the sums at the end. A thread restates its sums only when a block
 // of kRowDepth vectors holds a new maximum.
@@ -894,8 +896,9 @@ __device__ __forceinline__ float grad_element(const LogprobsGradLaunch& a, uint6
 }
 
 // Many classes: a CTA takes kGradThreads * kGradDepth vectors of one row. x and dx lie the
-// same distance from a 16-byte boundary (VEC), else it goes element by element. 4096 x 128000
-// bf16 with entropy: 383 us, 5.5 TB/s, bound by the memory's mixed reads and writes.
+// same distance from a 16-byte boundary (VEC), else it goes element by element (4096 x 32000
+// bf16: 107 us and 348 us). 4096 x 128000 bf16 with entropy: 379 us, 5.5 TB/s, bound by the
+// memory's mixed reads and writes; 405 us with the 48 registers that it takes unbounded.
 template <typename T, bool VEC, bool ENT>
 __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 2 ? 6 : 5) k_logprobs_grad(LogprobsGradLaunch a, uint32_t chunks) {
   constexpr int kV = Span<T>::kV;
@@ -950,10 +953,14 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 2 ? 6 : 5) k_logpro
 
 // Few classes: a CTA takes `rows` whole rows, their constants in shared memory. VEC: the
 // matrices are contiguous and aligned, so the rows are one run of 16-byte vectors whose
-// elements may lie in different rows; 1000000 x 7 f32: 16 us, 4.2 TB/s. magic = ceil(2^32 / classes): an element's row is the
+// elements may lie in different rows; 1000000 x 7 f32, inputs out of the L2: 20 us, 3.5 TB/s, the
+// rows' constants waited for before the first vector. Strided rows go element by element
+// (100000 x 100 bf16: 17 us and 49 us). magic = ceil(2^32 / classes): an element's row is the
 // high half of its index times magic, exactly, as index * classes < 2^32.
 constexpr uint32_t kGradRows = 1024;
-constexpr uint64_t kGradFewDepth = 8;  // 1000000 x 7 f32: 22.5 us; 4: 25.7 us, 2: 24.7 us, 1: 28.6 us
+// Vectors a thread: 8, 4 and 2 take 20, 24 and 24 us at 1000000 x 7 f32, 17, 18 and 20 us at
+// 27233 x 320 f32, 85, 93 and 94 us at 100000 x 1000 bf16, but 28, 27 and 29 us at 200000 x 100.
+constexpr uint64_t kGradFewDepth = 8;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kGradThreads) k_logprobs_grad_few(LogprobsGradLaunch a, uint32_t rows, uint32_t magic) {
@@ -1036,7 +1043,8 @@ uint32_t grid_of(uint64_t blocks, uint32_t per_sm) {
 constexpr uint64_t kFewClasses = 1024;
 
 // Parts a row: with fewer rows than four CTAs an SM, enough parts to make that many, of 4096
-// classes at least (a vector a thread).
+// classes at least (a vector a thread and more; top 5 of 8 x 128000 bf16: 7.7 us, 8.6 us from 2048
+// on, 7.1 us from 8192 on; of 1 x 16384: 6.4, 5.8 and 6.1 us).
 SplitRow split_of(uint64_t n, uint64_t classes) {
   SplitRow r = {1, classes, nullptr, nullptr};
   if (classes <= kFewClasses || n == 0 || n >= 148 * 4) return r;
@@ -1098,8 +1106,8 @@ cudaError_t launch_logprobs(const LogprobsLaunch& a, void* workspace, cudaStream
 }
 
 // Up to this many classes whole rows share CTAs where they are one run of vectors, since a CTA
-// of one row would have too little to do (50000 x 2050 bf16: 96 us and 171 us), else up to
-// kGradFewStrided.
+// of one row would have too little to do (50000 x 2050 bf16: 84 us and 173 us, x 4096 with
+// entropy 153 us and 233 us, but 20000 x 8192 135 us and 122 us), else up to kGradFewStrided.
 constexpr uint64_t kGradFew = 8192, kGradFewStrided = 1024;
 
 cudaError_t launch_logprobs_grad(const LogprobsGradLaunch& a, cudaStream_t s, int* nl) {
