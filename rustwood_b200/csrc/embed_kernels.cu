@@ -267,9 +267,8 @@ __global__ void __launch_bounds__(kCountThreads)
 // a frequent id is summed by many slots, and the order of every addition is fixed by the
 // ids and the sizes. Rows that no id names are zeroed by further CTAs of the same launch.
 // 65536 x 4096 bf16 into 128000 rows f32: 438 us for 2.6 GB, 5.9 TB/s; 473 us with the sort
-// and the join. Four CTAs an SM, as its launch bounds ask for, against two that 78 registers
-// leave: 36548 x 1128 bf16 into 8 rows 50 us and 54 us, 200000 x 1024 into 100 119 us and 127 us
-// (a 60000 x 502, whose vectors are narrow, takes 75 us either way).
+// and the join. Four CTAs an SM, as its launch bounds ask for, against the three that 78 registers
+// leave: 36548 x 1128 bf16 into 8 rows 50 us and 54 us, 200000 x 1024 into 100 119 us and 127 us.
 
 constexpr int kSumThreads = 256;
 constexpr int kSumDepth = 4;    // rows in flight per thread
@@ -864,11 +863,11 @@ int widest(uint64_t d, size_t elem) {
 // Chunks: enough for about 10 CTAs an SM where a row takes two warps or more, so that the
 // longest one does not decide the time (16: 36548 x 1128 bf16 into 8 rows 59 us instead of 50 us,
 // 65536 x 4096 bf16 into 128000 481 us instead of 475 us, f32 498 us instead of 506 us); for
-// narrower rows 4, whose slots are many and whose
-// runs then cross fewer chunks; no shorter than 8 positions (the partial sums would be more
-// than a quarter of the traffic) and no more than 32768 (k_embed_join looks at each). Their
-// length follows n, d and the type's widest vectors, not the V that strides and bases leave, so
-// that the order of the sums does not depend on the layout.
+// narrower rows 4, whose slots are many and whose runs then cross fewer chunks; no shorter than
+// 8 positions (the partial sums would be more than a quarter of the traffic) and no more than
+// 32768 (k_embed_join looks at each). Their length follows n, d and the type's widest vectors,
+// not the V that strides and bases leave, so that the order of the sums does not depend on the
+// layout.
 ChunkPlan chunk_plan(uint64_t n, uint64_t d, size_t elem, int V) {
   ChunkPlan c = {};
   chunk_columns(c, d, widest(d, elem));
